@@ -3,18 +3,27 @@ byte-identical compute the same bits.  Usage: python tools/codeobj_hash.py [path
 import hashlib, os, struct, subprocess, sys, tempfile
 
 
-def code_object(so):
+def code_objects(so):
+    """The gfx950 code objects of a library, one per translation unit, in link order (pocr_hip.hip first)."""
     data = open(so, "rb").read()
     magic = b"__CLANG_OFFLOAD_BUNDLE__"
-    at = data.find(magic)
-    n = struct.unpack_from("<Q", data, at + len(magic))[0]
-    p = at + len(magic) + 8
-    for _ in range(n):
-        off, size, tlen = struct.unpack_from("<QQQ", data, p); p += 24
-        triple = data[p:p + tlen].decode(); p += tlen
-        if "gfx950" in triple:
-            return data[at + off:at + off + size]
-    raise SystemExit(f"{so}: no gfx950 code object")
+    found, at = [], data.find(magic)
+    while at >= 0:
+        n = struct.unpack_from("<Q", data, at + len(magic))[0]
+        p = at + len(magic) + 8
+        for _ in range(n):
+            off, size, tlen = struct.unpack_from("<QQQ", data, p); p += 24
+            triple = data[p:p + tlen].decode(); p += tlen
+            if "gfx950" in triple:
+                found.append(data[at + off:at + off + size])
+        at = data.find(magic, p)
+    if not found:
+        raise SystemExit(f"{so}: no gfx950 code object")
+    return found
+
+
+def code_object(so):
+    return code_objects(so)[0]
 
 
 def text_section(elf):

@@ -16,7 +16,7 @@ import sys
 import tempfile
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from codeobj_hash import code_object  # noqa: E402
+from codeobj_hash import code_objects  # noqa: E402
 
 STORE = re.compile(r"^\s*buffer_store_(?:dwordx[34]|format_xyzw?|format_d16_xyzw)\s+v\[(\d+):(\d+)\],\s*(\S+),\s*s\[\d+:\d+\],\s*(\S+)")
 GSTORE = re.compile(r"^\s*(?:global|flat|scratch)_store_dwordx[34]\s+\S+,\s*v\[(\d+):(\d+)\]")
@@ -41,11 +41,12 @@ def scan(so):
     """-> (hits, stores of more than 64 bits, those with an SGPR offset).  Required distance to a VALU write of the data registers,
     as measured on gfx950 (tools/store_hazard_probe.hip): ONE wait state behind a buffer store with an SGPR offset (the case LLVM
     does not pad), TWO behind a buffer store with a literal offset and behind global / flat stores (LLVM pads those; checked anyway)."""
-    elf = code_object(so)
-    with tempfile.NamedTemporaryFile(suffix=".co") as f:
-        f.write(elf)
-        f.flush()
-        txt = subprocess.run(["/opt/rocm/lib/llvm/bin/llvm-objdump", "-d", "--no-show-raw-insn", f.name], capture_output=True, text=True, check=True).stdout
+    txt = ""
+    for elf in code_objects(so):                          # every translation unit's
+        with tempfile.NamedTemporaryFile(suffix=".co") as f:
+            f.write(elf)
+            f.flush()
+            txt += subprocess.run(["/opt/rocm/lib/llvm/bin/llvm-objdump", "-d", "--no-show-raw-insn", f.name], capture_output=True, text=True, check=True).stdout
     hits, n_stores, n_soff = [], 0, 0
     kernel = "?"
     lines = [l.split("//")[0] for l in txt.split("\n")]
