@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define POCR_ABI_VERSION 13
+#define POCR_ABI_VERSION 14
 #define POCR_NUM_SLOTS 4
 
 typedef struct pocr_engine pocr_engine;
@@ -369,6 +369,79 @@ int pocr_parsenet_last_ms(pocr_parsenet *p, float *ms);
  * lay below 2^-13 as a whole is run again - transparently, inside the same get_maps call - on the bf16x3 kernels (fp32's range)
  * of a second network created on first use; torch_parsenet.py:49-53 computes in plain fp32.  Returns the pages re-run so far. */
 int64_t pocr_parsenet_range_fallbacks(pocr_parsenet *p);
+
+/* ---- decoding operators (ABI 14; no reference counterpart: the reference's decoder keeps float32 keys / values of one batch as
+ * torch tensors, pero_ocr/ocr_engine/transformer.py:183-303, and decodes one token at a time) ----
+ * A paged cache of keys and values in bfloat16 or 8 bits, attention of the newest tokens of many sequences over it (single tokens,
+ * chains, trees of drafted tokens), and the scores of given tokens.  Unlike the rest of this interface they work on DEVICE memory
+ * of the caller and on the caller's stream (`stream`: a hipStream_t of `device_id`, NULL = its default stream): a call checks its arguments,
+ * enqueues and returns; nothing is allocated, copied or waited for, so a call may be captured into a graph and calls on
+ * different streams do not meet.  The calling thread's current device is left as it was.  No engine needed.
+ *
+ * Element types of q, k, v and logits: */
+enum { POCR_F32 = 0, POCR_BF16 = 1, POCR_F16 = 2 };
+/* Cache of one layer: k, v = [num_pages][kv_heads][page_size][head_dim], start aligned to 16 bytes; head_dim 32, 64, 128 or 256,
+ * page_size a power of two from 16 on.  Slot s = row s % page_size of page s / page_size.
+ * POCR_KV_FP8: e4m3 codes; every row (one token, one head) has an exponent in k_exp / v_exp [num_pages][kv_heads][page_size] and stands
+ * for code * 2^(exp - 127), exp = the smallest >= 27 with max |x| <= 448 * 2^(exp - 127).  Rounding is to nearest even: off by at most 2^-4 of
+ * the value, or 2^-10 * 2^(exp - 127) below 2^-6 * 2^(exp - 127).  An element that is not finite is stored as NaN and does not count for exp.
+ * POCR_KV_BF16: rounded to nearest even; k_exp and v_exp are not used. */
+enum { POCR_KV_BF16 = 0, POCR_KV_FP8 = 1 };
+typedef struct pocr_kv_pages {
+    void *k, *v;
+    uint8_t *k_exp, *v_exp;
+    int32_t num_pages, kv_heads, page_size, head_dim, format;
+} pocr_kv_pages;
+/* k, v [tokens][kv_heads][head_dim] with element strides per token and head (the last axis is contiguous) -> the rows of slots[tokens]
+ * (int64 when slots64, else int32).  A slot outside the cache (-1: padding) is skipped.  Slots of one call are distinct: a slot
+ * named twice holds a mixture of the rows given for it. */
+int pocr_kv_write(int device_id, void *stream, const pocr_kv_pages *pages, const void *k, const void *v, int32_t dtype, int64_t k_token_stride,
+                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void *slots, int32_t slots64, int64_t tokens);
+/* The rows of slots[tokens] -> k, v [tokens][kv_heads][head_dim] (contiguous, 16-byte aligned) as `dtype`, rounded to nearest even; a
+ * slot outside the cache reads as zeros. */
+int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const void *slots, int32_t slots64, int64_t tokens, void *k, void *v,
+                 int32_t dtype);
+/* Attention of the newest tokens of `seqs` sequences.  Sequence s: lengths[s] cached positions, position p in row p % page_size of page
+ * page_table[s * page_table_stride + p / page_size]; its new tokens are rows q_start[s] .. q_start[s + 1] - 1 of q, n of them, and their keys and
+ * values are already in the cache at the last n positions.  New token i sees all positions before these, and of these
+ *   mask NULL : 0 .. i (a chain);   else bit j of mask row i (words of 64 bits: bit j % 64 of word j / 64, row stride mask_stride words).
+ * A row whose mask leaves nothing gets out = 0 and lse = -inf.  Query head h reads key head h / (heads / kv_heads).
+ * A position beyond the page table or whose page id is outside the cache is absent: nobody sees it and it is never read.
+ * q_start is non-decreasing from 0 and ends at or below `tokens`; rows of out / lse behind q_start[seqs] are left as they were, or zeroed
+ * (lse: -inf) with zero_rest.  max_queries: the most new tokens of one sequence, if known (0: unknown): it shapes the launch, any
+ * value gives the same answer.  Sums and the softmax are in 32 bits. */
+typedef struct pocr_tree_attention_args {
+    const void *q;                    /* [tokens][heads][head_dim], element strides q_token_stride, q_head_stride */
+    void *out;                        /* [tokens][heads][head_dim] contiguous, 16-byte aligned */
+    float *lse;                       /* [tokens][heads] log of the sum of exp, or NULL */
+    const int32_t *page_table, *lengths, *q_start;
+    const uint64_t *mask;
+    void *workspace;                  /* pocr_tree_attention_workspace() bytes, 16-byte aligned; its contents mean nothing between calls */
+    int64_t workspace_bytes;
+    int64_t q_token_stride, q_head_stride, page_table_stride, mask_stride, tokens, max_queries;
+    int32_t dtype, seqs, heads, max_pages, mask_words, zero_rest;
+    float scale;                      /* of the scores, usually head_dim^-0.5 */
+} pocr_tree_attention_args;
+int64_t pocr_tree_attention_workspace(const pocr_kv_pages *pages, const pocr_tree_attention_args *args);
+int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *pages, const pocr_tree_attention_args *args);
+/* Scores of given tokens under logits [rows][classes] (row stride in elements): with p = softmax(row)
+ *   logprob [rows][given]   : log p[token] for tokens [rows][given] (int64 when tokens64, else int32); 0 for a negative token (padding),
+ *                             NaN for one beyond the classes
+ *   entropy [rows]          : -sum p log p
+ *   top_logprob, top_index [rows][top] : the `top` largest logits, 0 <= top <= min(64, classes), equal ones in the order of their index, NaN first
+ * A logit of -inf has probability 0; a row of nothing else has log probabilities -inf and entropy 0; a row with NaN or +inf has NaN.
+ * Sums are in 32 bits. */
+typedef struct pocr_token_logprobs_args {
+    const void *logits, *tokens;
+    float *logprob, *entropy, *top_logprob;
+    int32_t *top_index;
+    void *workspace;                  /* pocr_token_logprobs_workspace() bytes, 16-byte aligned; its contents mean nothing between calls */
+    int64_t workspace_bytes;
+    int64_t row_stride, rows;
+    int32_t dtype, classes, given, top, tokens64;
+} pocr_token_logprobs_args;
+int64_t pocr_token_logprobs_workspace(const pocr_token_logprobs_args *args);
+int pocr_token_logprobs(int device_id, void *stream, const pocr_token_logprobs_args *args);
 
 /* ---- measurement / test taps (not part of the reference surface) ----
  * Per-stage GPU time of the last pocr_run_* call in milliseconds, measured with HIP

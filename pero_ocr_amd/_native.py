@@ -14,7 +14,7 @@ import numpy as np
 from .netspec import NetSpec
 
 LIB_NAME = "libpocr_hip.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 UNIQUE_ID_BYTES = 128
 STAGE_NAMES = ("conv1", "conv2", "conv3", "conv4", "conv5", "conv6", "conv7", "conv8", "conv9",
                "agg", "lstm", "head", "ctc", "total")
@@ -40,6 +40,28 @@ CROP_SPEC_DTYPE = np.dtype([("x_min", "<f8"), ("x_max", "<f8"), ("lo", "<f8"), (
                             ("below", "<f8"), ("rot", "<f8", (4,)), ("mode", "<i4"), ("n_coef", "<i4"), ("coef_off", "<i4"),
                             ("knot_off", "<i4"), ("n_x", "<i4"), ("pad_", "<i4")])
 assert CROP_SPEC_DTYPE.itemsize == C.sizeof(CropSpec)
+
+class KvPages(C.Structure):
+    """pocr_kv_pages (include/pocr.h): one layer's paged cache of keys and values."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p), ("num_pages", C.c_int32),
+                ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("format", C.c_int32)]
+
+
+class TreeAttentionArgs(C.Structure):
+    """pocr_tree_attention_args (include/pocr.h)."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
+                ("q_start", C.c_void_p), ("mask", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+                ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("page_table_stride", C.c_int64), ("mask_stride", C.c_int64),
+                ("tokens", C.c_int64), ("max_queries", C.c_int64), ("dtype", C.c_int32), ("seqs", C.c_int32), ("heads", C.c_int32),
+                ("max_pages", C.c_int32), ("mask_words", C.c_int32), ("zero_rest", C.c_int32), ("scale", C.c_float)]
+
+
+class TokenLogprobsArgs(C.Structure):
+    """pocr_token_logprobs_args (include/pocr.h)."""
+    _fields_ = [("logits", C.c_void_p), ("tokens", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("top_logprob", C.c_void_p),
+                ("top_index", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("row_stride", C.c_int64), ("rows", C.c_int64),
+                ("dtype", C.c_int32), ("classes", C.c_int32), ("given", C.c_int32), ("top", C.c_int32), ("tokens64", C.c_int32)]
+
 
 ARCH_IDS = {"vgg_blstm_ctc": 0, "vgg_sa_ctc": 1, "vgg_sa_s2s": 2}
 
@@ -89,6 +111,13 @@ SYMBOLS = {
     "pocr_cropper_read_curves": (C.c_int, [C.c_void_p, C.POINTER(C.c_double), C.c_int64]),
     "pocr_cropper_last_ms": (C.c_float, [C.c_void_p]),
     "pocr_num_slots": (C.c_int, []),
+    "pocr_kv_write": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(KvPages), C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64,
+                                C.c_int64, C.c_void_p, C.c_int32, C.c_int64]),
+    "pocr_kv_read": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(KvPages), C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32]),
+    "pocr_tree_attention_workspace": (C.c_int64, [C.POINTER(KvPages), C.POINTER(TreeAttentionArgs)]),
+    "pocr_tree_attention": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(KvPages), C.POINTER(TreeAttentionArgs)]),
+    "pocr_token_logprobs_workspace": (C.c_int64, [C.POINTER(TokenLogprobsArgs)]),
+    "pocr_token_logprobs": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(TokenLogprobsArgs)]),
     "pocr_slot_stage_lines": (C.c_int, [C.c_void_p, C.c_int32, _u8p, _i64p, _i32p, C.c_int32, C.c_int32, C.c_int32]),
     "pocr_slot_stage_ragged": (C.c_int, [C.c_void_p, C.c_int32, _u8p, _i64p, _i32p, _i32p, C.c_int32, C.c_int32]),
     "pocr_slot_launch": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32]),

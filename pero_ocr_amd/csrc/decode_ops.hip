@@ -1,0 +1,218 @@
+// decode_ops.hip — C entries (include/pocr.h "decoding operators") of the stand-alone operators on device memory of the caller:
+// the paged key / value cache, attention of drafted tokens over it, scores of given tokens.  No engine, no host copies, no
+// allocation and no synchronisation: every call checks its arguments, enqueues on the caller's stream and returns.
+#include <hip/hip_runtime.h>
+#include <cstdarg>
+#include <cstdio>
+#include <type_traits>
+
+#include "../../include/pocr.h"
+#include "kv_cache.hpp"
+#include "token_logprobs.hpp"
+#include "tree_attention.hpp"
+
+namespace pocr {
+int set_error(const char *text);          // pocr_hip.hip: what pocr_last_error() returns on this thread; 1
+}
+
+using namespace pocr;
+
+static_assert((int)POCR_F32 == DT_F32 && (int)POCR_BF16 == DT_BF16 && (int)POCR_F16 == DT_F16, "element types");
+static_assert((int)POCR_KV_BF16 == KV_BF16 && (int)POCR_KV_FP8 == KV_FP8, "cache formats");
+
+namespace {
+
+int refuse(const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return set_error(buf);
+}
+
+// The caller's device for the length of a call (a thread's current device is left as it was).
+struct OnDevice {
+    int was = -1;
+    bool changed = false;
+    int enter(int device_id) {
+        int n = 0;
+        if (hipGetDeviceCount(&n) != hipSuccess || n == 0) return refuse("no HIP device available: this library has no CPU fallback");
+        if (device_id < 0 || device_id >= n) return refuse("device_id %d out of range (%d devices)", device_id, n);
+        if (hipGetDevice(&was) != hipSuccess) return refuse("hipGetDevice failed");
+        if (was != device_id) {
+            if (hipSetDevice(device_id) != hipSuccess) return refuse("hipSetDevice(%d) failed", device_id);
+            changed = true;
+        }
+        return 0;
+    }
+    ~OnDevice() { if (changed) (void)hipSetDevice(was); }
+};
+
+// the launch's own status: an error that some earlier call of the process left behind is not taken for this one's
+template <class Args> int launch(const char *what, void (*kernel)(Args), dim3 grid, dim3 block, void *stream, Args args) {
+    void *p[1] = {&args};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, p, 0, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : refuse("%s: launch failed: %s", what, hipGetErrorString(e));
+}
+
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int elem_size(int dtype) { return dtype == POCR_F32 ? 4 : 2; }
+bool known_dtype(int dtype) { return dtype == POCR_F32 || dtype == POCR_BF16 || dtype == POCR_F16; }
+
+int page_shift(const pocr_kv_pages *c) { int s = 0; while ((1 << s) < c->page_size) ++s; return s; }
+
+int check_pages(const pocr_kv_pages *c) {
+    if (!c || !c->k || !c->v) return refuse("NULL cache");
+    if (c->format != POCR_KV_BF16 && c->format != POCR_KV_FP8) return refuse("cache format %d: POCR_KV_BF16 or POCR_KV_FP8", c->format);
+    if (c->format == POCR_KV_FP8 && (!c->k_exp || !c->v_exp)) return refuse("an 8-bit cache needs k_exp and v_exp");
+    if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return refuse("head_dim %d: 32, 64, 128 or 256", c->head_dim);
+    if (c->page_size < 16 || (c->page_size & (c->page_size - 1)) || c->page_size > 1 << 30) return refuse("page_size %d: a power of two from 16 on", c->page_size);
+    if (c->num_pages < 1 || c->kv_heads < 1) return refuse("num_pages and kv_heads must be positive (got %d, %d)", c->num_pages, c->kv_heads);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return refuse("the cache must start at a multiple of 16 bytes");
+    return 0;
+}
+
+int check_rows(const pocr_kv_pages *c, int64_t tokens, const char *what) {
+    if (tokens < 0) return refuse("%s: tokens %lld", what, (long long)tokens);
+    if (tokens > ((int64_t)1 << 31) / (2 * (int64_t)c->kv_heads) - 128) return refuse("%s: 2 * tokens * kv_heads must stay below 2^31", what);
+    return 0;
+}
+
+template <int DT, int FMT, bool VEC> int write_by_dim(dim3 (*grid)(uint32_t, int), int D, void *stream, const KvWriteArgs &a) {
+    const char *w = "pocr_kv_write";
+    switch (D) {
+        case 32: return launch(w, kv_write_kernel<DT, FMT, 32, VEC>, grid(a.rows, 32), dim3(256), stream, a);
+        case 64: return launch(w, kv_write_kernel<DT, FMT, 64, VEC>, grid(a.rows, 64), dim3(256), stream, a);
+        case 128: return launch(w, kv_write_kernel<DT, FMT, 128, VEC>, grid(a.rows, 128), dim3(256), stream, a);
+        default: return launch(w, kv_write_kernel<DT, FMT, 256, VEC>, grid(a.rows, 256), dim3(256), stream, a);
+    }
+}
+
+template <int DT, int FMT> int read_by_dim(dim3 (*grid)(uint32_t, int), int D, void *stream, const KvReadArgs &a) {
+    const char *w = "pocr_kv_read";
+    switch (D) {
+        case 32: return launch(w, kv_read_kernel<DT, FMT, 32>, grid(a.rows, 32), dim3(256), stream, a);
+        case 64: return launch(w, kv_read_kernel<DT, FMT, 64>, grid(a.rows, 64), dim3(256), stream, a);
+        case 128: return launch(w, kv_read_kernel<DT, FMT, 128>, grid(a.rows, 128), dim3(256), stream, a);
+        default: return launch(w, kv_read_kernel<DT, FMT, 256>, grid(a.rows, 256), dim3(256), stream, a);
+    }
+}
+
+dim3 row_grid(uint32_t rows, int D) { const uint32_t per = 256 / (D / 8); return dim3((rows + per - 1) / per); }
+
+template <int DT, int FMT> int attend_by_dim(int D, dim3 grid, void *stream, const TreeAttnArgs &a) {
+    const char *w = "pocr_tree_attention";
+    switch (D) {
+        case 32: return launch(w, tree_attention_kernel<DT, FMT, 32>, grid, dim3(64), stream, a);
+        case 64: return launch(w, tree_attention_kernel<DT, FMT, 64>, grid, dim3(64), stream, a);
+        case 128: return launch(w, tree_attention_kernel<DT, FMT, 128>, grid, dim3(64), stream, a);
+        default: return launch(w, tree_attention_kernel<DT, FMT, 256>, grid, dim3(64), stream, a);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int pocr_kv_write(int device_id, void *stream, const pocr_kv_pages *c, const void *k, const void *v, int32_t dtype, int64_t k_token_stride,
+                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void *slots, int32_t slots64, int64_t tokens) {
+    if (check_pages(c) || check_rows(c, tokens, "pocr_kv_write")) return 1;
+    if (!known_dtype(dtype)) return refuse("pocr_kv_write: dtype %d", dtype);
+    if (tokens == 0) return 0;
+    if (!k || !v || !slots) return refuse("pocr_kv_write: NULL pointer");
+    const int es = elem_size(dtype);
+    if (!aligned(k, es) || !aligned(v, es) || !aligned(slots, slots64 ? 8 : 4)) return refuse("pocr_kv_write: a pointer is not aligned to its element");
+    OnDevice dev;
+    if (dev.enter(device_id)) return 1;
+    KvWriteArgs a{c->k, c->v, c->k_exp, c->v_exp, k, v, slots, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
+                  c->num_pages, c->kv_heads, page_shift(c), (uint32_t)(tokens * 2 * c->kv_heads), slots64};
+    // 16-byte loads where every row starts at a multiple of 16 bytes, single elements otherwise
+    const bool vec = aligned(k, 16) && aligned(v, 16) && (k_token_stride * es) % 16 == 0 && (k_head_stride * es) % 16 == 0 &&
+                     (v_token_stride * es) % 16 == 0 && (v_head_stride * es) % 16 == 0;
+    auto go = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (c->format == POCR_KV_FP8) return vec ? write_by_dim<DT, KV_FP8, true>(row_grid, c->head_dim, stream, a) : write_by_dim<DT, KV_FP8, false>(row_grid, c->head_dim, stream, a);
+        return vec ? write_by_dim<DT, KV_BF16, true>(row_grid, c->head_dim, stream, a) : write_by_dim<DT, KV_BF16, false>(row_grid, c->head_dim, stream, a);
+    };
+    if (dtype == POCR_F32) return go(std::integral_constant<int, DT_F32>());
+    if (dtype == POCR_BF16) return go(std::integral_constant<int, DT_BF16>());
+    return go(std::integral_constant<int, DT_F16>());
+}
+
+int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *c, const void *slots, int32_t slots64, int64_t tokens, void *k, void *v, int32_t dtype) {
+    if (check_pages(c) || check_rows(c, tokens, "pocr_kv_read")) return 1;
+    if (!known_dtype(dtype)) return refuse("pocr_kv_read: dtype %d", dtype);
+    if (tokens == 0) return 0;
+    if (!k || !v || !slots) return refuse("pocr_kv_read: NULL pointer");
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, slots64 ? 8 : 4)) return refuse("pocr_kv_read: k and v must start at a multiple of 16 bytes");
+    OnDevice dev;
+    if (dev.enter(device_id)) return 1;
+    KvReadArgs a{c->k, c->v, c->k_exp, c->v_exp, k, v, slots, c->num_pages, c->kv_heads, page_shift(c), (uint32_t)(tokens * 2 * c->kv_heads), slots64};
+    auto go = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return c->format == POCR_KV_FP8 ? read_by_dim<DT, KV_FP8>(row_grid, c->head_dim, stream, a) : read_by_dim<DT, KV_BF16>(row_grid, c->head_dim, stream, a);
+    };
+    if (dtype == POCR_F32) return go(std::integral_constant<int, DT_F32>());
+    if (dtype == POCR_BF16) return go(std::integral_constant<int, DT_BF16>());
+    return go(std::integral_constant<int, DT_F16>());
+}
+
+int64_t pocr_tree_attention_workspace(const pocr_kv_pages *, const pocr_tree_attention_args *) { return 0; }
+
+int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
+    if (check_pages(c)) return 1;
+    if (!t) return refuse("pocr_tree_attention: NULL arguments");
+    if (!known_dtype(t->dtype)) return refuse("pocr_tree_attention: dtype %d", t->dtype);
+    if (t->tokens < 0 || t->tokens > 0x7fffffff || t->seqs < 0) return refuse("pocr_tree_attention: tokens %lld, seqs %d", (long long)t->tokens, t->seqs);
+    if (t->heads < 1 || t->heads % c->kv_heads) return refuse("pocr_tree_attention: heads %d must be a multiple of the cache's %d key heads", t->heads, c->kv_heads);
+    if (t->heads > 65535) return refuse("pocr_tree_attention: heads %d exceeds 65535", t->heads);
+    if (t->max_pages < 0) return refuse("pocr_tree_attention: max_pages %d", t->max_pages);
+    if (t->mask && t->mask_words < 1) return refuse("pocr_tree_attention: mask_words %d", t->mask_words);
+    if (t->tokens == 0) return 0;
+    if (t->seqs == 0) return refuse("pocr_tree_attention: tokens without a sequence");
+    if (!t->q || !t->out || !t->lengths || !t->q_start || (t->max_pages > 0 && !t->page_table)) return refuse("pocr_tree_attention: NULL pointer");
+    const int es = elem_size(t->dtype);
+    if (!aligned(t->q, es) || !aligned(t->out, 16) || !aligned(t->lse, 4) || !aligned(t->mask, 8) || !aligned(t->lengths, 4) || !aligned(t->q_start, 4) || !aligned(t->page_table, 4))
+        return refuse("pocr_tree_attention: a pointer is not aligned to its element (out: to 16 bytes)");
+    OnDevice dev;
+    if (dev.enter(device_id)) return 1;
+    TreeAttnArgs a{t->q, c->k, c->v, c->k_exp, c->v_exp, t->page_table, t->lengths, t->q_start, t->mask, t->out, t->lse, t->q_token_stride, t->q_head_stride,
+                   t->page_table_stride, t->mask_stride, t->tokens, t->seqs, t->heads, c->kv_heads, c->num_pages, page_shift(c), t->max_pages, t->mask_words,
+                   t->zero_rest, t->scale};
+    int64_t most = t->max_queries > 0 && t->max_queries < t->tokens ? t->max_queries : t->tokens;
+    if (most > 64) most = 64;
+    const dim3 grid((unsigned)t->seqs, (unsigned)t->heads, (unsigned)most);
+    auto go = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return c->format == POCR_KV_FP8 ? attend_by_dim<DT, KV_FP8>(c->head_dim, grid, stream, a) : attend_by_dim<DT, KV_BF16>(c->head_dim, grid, stream, a);
+    };
+    if (t->dtype == POCR_F32) return go(std::integral_constant<int, DT_F32>());
+    if (t->dtype == POCR_BF16) return go(std::integral_constant<int, DT_BF16>());
+    return go(std::integral_constant<int, DT_F16>());
+}
+
+int64_t pocr_token_logprobs_workspace(const pocr_token_logprobs_args *) { return 0; }
+
+int pocr_token_logprobs(int device_id, void *stream, const pocr_token_logprobs_args *t) {
+    if (!t) return refuse("pocr_token_logprobs: NULL arguments");
+    if (!known_dtype(t->dtype)) return refuse("pocr_token_logprobs: dtype %d", t->dtype);
+    if (t->rows < 0 || t->rows > 0x7fffffff) return refuse("pocr_token_logprobs: rows %lld", (long long)t->rows);
+    if (t->classes < 1 || t->classes > 1 << 30) return refuse("pocr_token_logprobs: classes %d", t->classes);
+    if (t->given < 0) return refuse("pocr_token_logprobs: given %d", t->given);
+    if (t->top < 0 || t->top > LP_MAX_TOP || t->top > t->classes) return refuse("pocr_token_logprobs: top %d must be in 0..%d and at most the classes", t->top, LP_MAX_TOP);
+    if (t->rows == 0) return 0;
+    if (!t->logits || !t->entropy || (t->given > 0 && (!t->tokens || !t->logprob)) || (t->top > 0 && (!t->top_logprob || !t->top_index)))
+        return refuse("pocr_token_logprobs: NULL pointer");
+    if (!aligned(t->logits, elem_size(t->dtype)) || !aligned(t->tokens, t->tokens64 ? 8 : 4)) return refuse("pocr_token_logprobs: a pointer is not aligned to its element");
+    OnDevice dev;
+    if (dev.enter(device_id)) return 1;
+    LogprobArgs a{t->logits, t->row_stride, t->tokens, t->logprob, t->entropy, t->top_logprob, t->top_index, t->rows, t->classes, t->given, t->top, t->tokens64};
+    const char *w = "pocr_token_logprobs";
+    const dim3 grid((unsigned)t->rows), block(256);
+    if (t->dtype == POCR_F32) return launch(w, token_logprobs_kernel<DT_F32>, grid, block, stream, a);
+    if (t->dtype == POCR_BF16) return launch(w, token_logprobs_kernel<DT_BF16>, grid, block, stream, a);
+    return launch(w, token_logprobs_kernel<DT_F16>, grid, block, stream, a);
+}
+
+}  // extern "C"

@@ -37,8 +37,14 @@
 using namespace pocr;
 
 namespace {
-
 thread_local std::string g_err;
+}
+
+namespace pocr {
+__attribute__((visibility("hidden"))) int set_error(const char *text) { g_err = text; return 1; }      // (decode_ops.hip)
+}
+
+namespace {
 
 int fail(const char *fmt, ...) {
     char buf[1024];
