@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <cstdarg>
 #include <cstdio>
+#include <algorithm>
 #include <type_traits>
 
 #include "../../include/pocr.h"
@@ -70,6 +71,7 @@ int check_pages(const pocr_kv_pages *c) {
     if (c->page_size < 16 || (c->page_size & (c->page_size - 1)) || c->page_size > 1 << 30) return refuse("page_size %d: a power of two from 16 on", c->page_size);
     if (c->num_pages < 1 || c->kv_heads < 1) return refuse("num_pages and kv_heads must be positive (got %d, %d)", c->num_pages, c->kv_heads);
     if (!aligned(c->k, 16) || !aligned(c->v, 16)) return refuse("the cache must start at a multiple of 16 bytes");
+    if (c->format == POCR_KV_FP8 && (!aligned(c->k_exp, 4) || !aligned(c->v_exp, 4))) return refuse("k_exp and v_exp must start at a multiple of 4 bytes");
     return 0;
 }
 
@@ -101,14 +103,52 @@ template <int DT, int FMT> int read_by_dim(dim3 (*grid)(uint32_t, int), int D, v
 
 dim3 row_grid(uint32_t rows, int D) { const uint32_t per = 256 / (D / 8); return dim3((rows + per - 1) / per); }
 
-template <int DT, int FMT> int attend_by_dim(int D, dim3 grid, void *stream, const TreeAttnArgs &a) {
+// How the work of one attention call is cut.
+struct AttendPlan { int rt, tiles, nsplit, waves; int64_t groups; };
+
+AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
+    AttendPlan p;
+    const int64_t most = t->max_queries > 0 && t->max_queries < t->tokens ? t->max_queries : t->tokens;
+    const int64_t rows = most * (t->heads / c->kv_heads), pairs = (int64_t)t->seqs * c->kv_heads;
+    p.rt = rows > 16 && c->head_dim <= 128 ? 2 : 1;
+    p.tiles = (int)std::min<int64_t>((rows + 16 * p.rt - 1) / (16 * p.rt), 1024);
+    const int64_t units = pairs * p.tiles, blocks = (((int64_t)t->max_pages << page_shift(c)) + 31) / 32;
+    const int64_t want = (512 + units - 1) / units, most_splits = std::max<int64_t>(1, blocks / 8);
+    p.nsplit = (int)std::min<int64_t>(std::min(want, most_splits), 128);
+    p.waves = units >= 2048 ? 1 : TA_WAVES;
+    p.groups = (pairs * p.nsplit + 7) / 8 * 8 * p.tiles;
+    return p;
+}
+
+template <int DT, int FMT, int D> int attend(const AttendPlan &p, void *stream, const TreeAttnArgs &a) {
     const char *w = "pocr_tree_attention";
+    const dim3 grid((unsigned)p.groups), block(64 * p.waves);
+    constexpr int RT = D <= 128 ? 2 : 1;
+    const int rc = p.rt == 1 ? launch(w, tree_attention_kernel<DT, FMT, D, 1>, grid, block, stream, a) : launch(w, tree_attention_kernel<DT, FMT, D, RT>, grid, block, stream, a);
+    if (rc || p.nsplit == 1) return rc;
+    return launch(w, tree_attention_join_kernel<DT, D>, dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), stream, a);
+}
+
+template <int DT, int FMT> int attend_by_dim(int D, const AttendPlan &p, void *stream, const TreeAttnArgs &a) {
     switch (D) {
-        case 32: return launch(w, tree_attention_kernel<DT, FMT, 32>, grid, dim3(64), stream, a);
-        case 64: return launch(w, tree_attention_kernel<DT, FMT, 64>, grid, dim3(64), stream, a);
-        case 128: return launch(w, tree_attention_kernel<DT, FMT, 128>, grid, dim3(64), stream, a);
-        default: return launch(w, tree_attention_kernel<DT, FMT, 256>, grid, dim3(64), stream, a);
+        case 32: return attend<DT, FMT, 32>(p, stream, a);
+        case 64: return attend<DT, FMT, 64>(p, stream, a);
+        case 128: return attend<DT, FMT, 128>(p, stream, a);
+        default: return attend<DT, FMT, 256>(p, stream, a);
     }
+}
+
+int check_attention(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
+    if (check_pages(c)) return 1;
+    if (!t) return refuse("pocr_tree_attention: NULL arguments");
+    if (!known_dtype(t->dtype)) return refuse("pocr_tree_attention: dtype %d", t->dtype);
+    if (t->tokens < 0 || t->tokens > 0x7fffffff || t->seqs < 0) return refuse("pocr_tree_attention: tokens %lld, seqs %d", (long long)t->tokens, t->seqs);
+    if (t->heads < 1 || t->heads % c->kv_heads) return refuse("pocr_tree_attention: heads %d must be a multiple of the cache's %d key heads", t->heads, c->kv_heads);
+    if (t->max_pages < 0) return refuse("pocr_tree_attention: max_pages %d", t->max_pages);
+    if (t->tokens > 0 && t->seqs == 0) return refuse("pocr_tree_attention: tokens without a sequence");
+    if ((int64_t)t->seqs * c->kv_heads > 1 << 20 || t->tokens * t->heads > 0x7fffffff)
+        return refuse("pocr_tree_attention: seqs * kv_heads exceeds 2^20 or tokens * heads 2^31");
+    return 0;
 }
 
 }  // namespace
@@ -158,34 +198,34 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *c, const void
     return go(std::integral_constant<int, DT_F16>());
 }
 
-int64_t pocr_tree_attention_workspace(const pocr_kv_pages *, const pocr_tree_attention_args *) { return 0; }
+int64_t pocr_tree_attention_workspace(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
+    if (check_attention(c, t)) return -1;
+    if (t->tokens == 0) return 0;
+    const AttendPlan p = attend_plan(c, t);
+    return p.nsplit == 1 ? 0 : (int64_t)p.nsplit * t->tokens * t->heads * (c->head_dim + 2) * 4;
+}
 
 int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
-    if (check_pages(c)) return 1;
-    if (!t) return refuse("pocr_tree_attention: NULL arguments");
-    if (!known_dtype(t->dtype)) return refuse("pocr_tree_attention: dtype %d", t->dtype);
-    if (t->tokens < 0 || t->tokens > 0x7fffffff || t->seqs < 0) return refuse("pocr_tree_attention: tokens %lld, seqs %d", (long long)t->tokens, t->seqs);
-    if (t->heads < 1 || t->heads % c->kv_heads) return refuse("pocr_tree_attention: heads %d must be a multiple of the cache's %d key heads", t->heads, c->kv_heads);
-    if (t->heads > 65535) return refuse("pocr_tree_attention: heads %d exceeds 65535", t->heads);
-    if (t->max_pages < 0) return refuse("pocr_tree_attention: max_pages %d", t->max_pages);
+    if (check_attention(c, t)) return 1;
     if (t->mask && t->mask_words < 1) return refuse("pocr_tree_attention: mask_words %d", t->mask_words);
     if (t->tokens == 0) return 0;
-    if (t->seqs == 0) return refuse("pocr_tree_attention: tokens without a sequence");
     if (!t->q || !t->out || !t->lengths || !t->q_start || (t->max_pages > 0 && !t->page_table)) return refuse("pocr_tree_attention: NULL pointer");
     const int es = elem_size(t->dtype);
     if (!aligned(t->q, es) || !aligned(t->out, 16) || !aligned(t->lse, 4) || !aligned(t->mask, 8) || !aligned(t->lengths, 4) || !aligned(t->q_start, 4) || !aligned(t->page_table, 4))
         return refuse("pocr_tree_attention: a pointer is not aligned to its element (out: to 16 bytes)");
+    const AttendPlan p = attend_plan(c, t);
+    const int64_t need = p.nsplit == 1 ? 0 : (int64_t)p.nsplit * t->tokens * t->heads * (c->head_dim + 2) * 4;
+    if (need > 0 && (!t->workspace || !aligned(t->workspace, 16) || t->workspace_bytes < need))
+        return refuse("pocr_tree_attention: a workspace of %lld bytes, aligned to 16, is needed (pocr_tree_attention_workspace)", (long long)need);
     OnDevice dev;
     if (dev.enter(device_id)) return 1;
-    TreeAttnArgs a{t->q, c->k, c->v, c->k_exp, c->v_exp, t->page_table, t->lengths, t->q_start, t->mask, t->out, t->lse, t->q_token_stride, t->q_head_stride,
-                   t->page_table_stride, t->mask_stride, t->tokens, t->seqs, t->heads, c->kv_heads, c->num_pages, page_shift(c), t->max_pages, t->mask_words,
-                   t->zero_rest, t->scale};
-    int64_t most = t->max_queries > 0 && t->max_queries < t->tokens ? t->max_queries : t->tokens;
-    if (most > 64) most = 64;
-    const dim3 grid((unsigned)t->seqs, (unsigned)t->heads, (unsigned)most);
+    const bool q_vec = aligned(t->q, 16) && (t->q_token_stride * es) % 16 == 0 && (t->q_head_stride * es) % 16 == 0;
+    TreeAttnArgs a{t->q, c->k, c->v, c->k_exp, c->v_exp, t->page_table, t->lengths, t->q_start, t->mask, t->out, t->lse, static_cast<float *>(t->workspace),
+                   t->q_token_stride, t->q_head_stride, t->page_table_stride, t->mask_stride, t->tokens, t->seqs, t->heads, c->kv_heads, c->num_pages, page_shift(c),
+                   t->max_pages, t->mask_words, t->zero_rest, p.nsplit, p.tiles, q_vec, t->scale};
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        return c->format == POCR_KV_FP8 ? attend_by_dim<DT, KV_FP8>(c->head_dim, grid, stream, a) : attend_by_dim<DT, KV_BF16>(c->head_dim, grid, stream, a);
+        return c->format == POCR_KV_FP8 ? attend_by_dim<DT, KV_FP8>(c->head_dim, p, stream, a) : attend_by_dim<DT, KV_BF16>(c->head_dim, p, stream, a);
     };
     if (t->dtype == POCR_F32) return go(std::integral_constant<int, DT_F32>());
     if (t->dtype == POCR_BF16) return go(std::integral_constant<int, DT_BF16>());

@@ -231,7 +231,9 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
             mask.data_ptr() if mask is not None else None, None, 0, qs[0], qs[1], ps[0], mask.stride(0) if mask is not None else 0, tokens, int(max_queries),
             _DTYPES[q.dtype], seqs, heads, page_table.shape[1], mask.shape[1] if mask is not None else 0, fresh, dim ** -0.5 if scale is None else float(scale))
         need = lib.pocr_tree_attention_workspace(n, args)
-        if need > 0:
+        if need < 0:
+            _fail("pocr_tree_attention")
+        if need:
             scratch = torch.empty(need, dtype=torch.uint8, device=device)
             args.workspace, args.workspace_bytes = scratch.data_ptr(), need
         if lib.pocr_tree_attention(device.index, _stream(device), n, args):
@@ -269,7 +271,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
             logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), None, 0,
             logits.stride(0), rows, _DTYPES[logits.dtype], classes, tokens.shape[1] if tokens.dim() == 2 else 1, top, tokens.dtype is torch.int64)
         need = lib.pocr_token_logprobs_workspace(args)
-        if need > 0:
+        if need < 0:
+            _fail("pocr_token_logprobs")
+        if need:
             scratch = torch.empty(need, dtype=torch.uint8, device=device)
             args.workspace, args.workspace_bytes = scratch.data_ptr(), need
         if lib.pocr_token_logprobs(device.index, _stream(device), args):
