@@ -151,6 +151,16 @@ int check_attention(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
     return 0;
 }
 
+template <int DT> int score(void *stream, const LogprobArgs &a) {
+    const char *w = "pocr_token_logprobs";
+    const unsigned rows = (unsigned)a.rows;
+    if (a.C <= 256) return launch(w, token_logprobs_few_kernel<DT, 16>, dim3((rows + 15) / 16), dim3(256), stream, a);
+    if (a.C <= 512) return launch(w, token_logprobs_few_kernel<DT, 32>, dim3((rows + 15) / 16), dim3(256), stream, a);
+    if (a.C <= 4096) return launch(w, token_logprobs_kernel<DT, 64>, dim3(rows), dim3(64), stream, a);
+    if (a.C <= 32768) return launch(w, token_logprobs_kernel<DT, 256>, dim3(rows), dim3(256), stream, a);
+    return launch(w, token_logprobs_kernel<DT, 1024>, dim3(rows), dim3(1024), stream, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -247,12 +257,11 @@ int pocr_token_logprobs(int device_id, void *stream, const pocr_token_logprobs_a
     if (!aligned(t->logits, elem_size(t->dtype)) || !aligned(t->tokens, t->tokens64 ? 8 : 4)) return refuse("pocr_token_logprobs: a pointer is not aligned to its element");
     OnDevice dev;
     if (dev.enter(device_id)) return 1;
-    LogprobArgs a{t->logits, t->row_stride, t->tokens, t->logprob, t->entropy, t->top_logprob, t->top_index, t->rows, t->classes, t->given, t->top, t->tokens64};
-    const char *w = "pocr_token_logprobs";
-    const dim3 grid((unsigned)t->rows), block(256);
-    if (t->dtype == POCR_F32) return launch(w, token_logprobs_kernel<DT_F32>, grid, block, stream, a);
-    if (t->dtype == POCR_BF16) return launch(w, token_logprobs_kernel<DT_BF16>, grid, block, stream, a);
-    return launch(w, token_logprobs_kernel<DT_F16>, grid, block, stream, a);
+    LogprobArgs a{t->logits, t->row_stride, t->tokens, t->logprob, t->entropy, t->top_logprob, t->top_index, t->rows, t->classes, t->given, t->top, t->tokens64,
+                  t->dtype};
+    if (t->dtype == POCR_F32) return score<DT_F32>(stream, a);
+    if (t->dtype == POCR_BF16) return score<DT_BF16>(stream, a);
+    return score<DT_F16>(stream, a);
 }
 
 }  // extern "C"

@@ -21,7 +21,7 @@ struct LogprobArgs {
     float *top_logprob;               // [rows][top]
     int32_t *top_index;               // [rows][top]
     int64_t rows;
-    int32_t C, given, top, tokens64;
+    int32_t C, given, top, tokens64, dtype;
 };
 
 constexpr int LP_MAX_TOP = 64;
@@ -37,60 +37,284 @@ __device__ __forceinline__ float lp_value(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// One workgroup per row; the alternatives one after the other.
-template <int DT>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
+
+// ---- few classes: 16 lanes per row, NV logits in a lane's registers (class lane + 16 i), four rows per wave, so that a reduction of four
+// steps serves four rows.  The alternatives are picked one after the other: the largest key, then the lowest class that has it.
+__device__ __forceinline__ uint32_t max16(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));       // row_ror:8, 4, 2, 1: within 16 lanes
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float sum16(float x) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false));
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, false));
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, false));
+}
+
+__device__ __forceinline__ void lp_given(const LogprobArgs &a, int64_t r, int first, int step, float base, float logz, bool none) {
+    for (int g = first; g < a.given; g += step) {
+        const int64_t at = r * a.given + g;
+        const int64_t t = a.tokens64 ? static_cast<const int64_t *>(a.tokens)[at] : static_cast<const int32_t *>(a.tokens)[at];
+        float lp = 0.f;
+        if (t >= a.C) lp = __builtin_nanf("");
+        else if (t >= 0) {
+            const int64_t e = r * a.stride + t;
+            const float v = a.dtype == DT_F32 ? static_cast<const float *>(a.x)[e] : a.dtype == DT_BF16 ? (float)static_cast<const __bf16 *>(a.x)[e] : (float)static_cast<const _Float16 *>(a.x)[e];
+            lp = none ? -INFINITY : (v - base) - logz;
+        }
+        a.logprob[at] = lp;
+    }
+}
+
+template <int DT, int NV>
+__global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) {
     using T = typename ElemOf<DT>::type;
-    __shared__ float red[8];
-    __shared__ unsigned long long best[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x & 15;
+    const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (r >= a.rows) return;                                    // (whole groups of 16 lanes)
     const T *x = static_cast<const T *>(a.x) + r * a.stride;
-    float m = -INFINITY;
-    int bad = 0;
-    for (int c = tid; c < a.C; c += 256) { const float v = (float)x[c]; m = fmaxf(m, v); bad |= v != v; }
-    for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    if (lane == 0) red[wave] = m;
-    bad = __syncthreads_or(bad);
-    m = bad ? __builtin_nanf("") : fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    uint32_t key[NV];
+    float v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = lane + 16 * i < a.C ? (float)x[lane + 16 * i] : 0.f;
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        key[i] = lane + 16 * i < a.C ? lp_key(v[i]) : 0u;       // (below the key of -inf)
+        best = max(best, key[i]);
+    }
+    best = max16(best);
+    const float m = lp_value(best);
     const float base = m == -INFINITY ? 0.f : m;
     float z = 0.f, e = 0.f;
-    for (int c = tid; c < a.C; c += 256) {
-        const float d = (float)x[c] - base, p = expf(d);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const float d = v[i] - base, p = lane + 16 * i < a.C ? __builtin_amdgcn_exp2f(d * 1.44269504088896f) : 0.f;
         z += p;
         e += p == 0.f ? 0.f : p * d;
     }
-    for (int off = 32; off >= 1; off >>= 1) { z += __shfl_xor(z, off, 64); e += __shfl_xor(e, off, 64); }
-    __syncthreads();
-    if (lane == 0) { red[wave] = z; red[4 + wave] = e; }
-    __syncthreads();
-    z = red[0] + red[1] + red[2] + red[3];
-    e = red[4] + red[5] + red[6] + red[7];
-    const float logz = logf(z);
-    auto logp = [&](float v) { return z == 0.f ? -INFINITY : (v - base) - logz; };
-    if (tid == 0) a.entropy[r] = z == 0.f ? 0.f : logz - e / z;
-    for (int g = tid; g < a.given; g += 256) {
-        const int64_t at = r * a.given + g;
-        const int64_t t = a.tokens64 ? static_cast<const int64_t *>(a.tokens)[at] : static_cast<const int32_t *>(a.tokens)[at];
-        a.logprob[at] = t < 0 ? 0.f : t >= a.C ? __builtin_nanf("") : logp((float)x[t]);
+    z = sum16(z);
+    e = sum16(e);
+    const bool none = z == 0.f;
+    const float logz = __builtin_amdgcn_logf(z) * 0.693147180559945f;
+    if (lane == 0) a.entropy[r] = none ? 0.f : logz - e / z;
+    lp_given(a, r, lane, 16, base, logz, none);
+    for (int t = 0; t < a.top; ++t) {
+        if (t) {
+            best = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) best = max(best, key[i]);
+            best = max16(best);
+        }
+        uint32_t low = 0;                                       // ~class: the largest is the lowest class
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i) low = key[i] == best ? ~(uint32_t)(lane + 16 * i) : low;
+        low = max16(low);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = ~low == (uint32_t)(lane + 16 * i) ? 0u : key[i];
+        if (lane == 0) {
+            a.top_logprob[r * a.top + t] = none ? -INFINITY : (lp_value(best) - base) - logz;
+            a.top_index[r * a.top + t] = (int32_t)~low;
+        }
     }
-    unsigned long long last = ~0ull;                            // (key, ~index) of the previous alternative
-    for (int i = 0; i < a.top; ++i) {
+}
+
+// ---- many classes: a workgroup of B threads per row, one pass over it in 16-byte pieces; thread t takes pieces t, t + B, ... and keeps the
+// running maximum, sum and weighted sum of its own.  The alternatives cost no second pass: a row's k best lie with the threads whose
+// own maximum is among the k largest, so only these threads' pieces (k of B shares) are read again, and of them only what reaches the k-th
+// largest maximum T is kept and ranked.  Where many threads share T (equal logits, rows that are masked but for a few classes) the
+// numbers above T are kept and the lowest classes equal to T are found by reading the row from its start.  What does not fit
+// the list of candidates, and rows with NaN or +inf, take one pass per alternative.
+constexpr int LP_CAND = 1024, LP_SLACK = 32;
+
+template <int DT, int V> __device__ __forceinline__ void lp_load(const void *p, float (&x)[V]) {
+    using T = typename ElemOf<DT>::type;
+    alignas(16) T t[V];
+    *reinterpret_cast<kv_u32x4 *>(t) = *static_cast<const kv_u32x4 *>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = (float)t[i];
+}
+
+template <int DT, int B>
+__global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
+    using T = typename ElemOf<DT>::type;
+    constexpr int V = 16 / sizeof(T), W = B / 64, U = 4;
+    static_assert(B <= LP_CAND && LP_MAX_TOP <= B, "the list of candidates; a maximum per thread for every alternative");
+    __shared__ float red[3][W];
+    __shared__ uint32_t maxima[B];
+    __shared__ uint32_t picked[B];                              // threads whose pieces are read again
+    __shared__ unsigned long long cand[LP_CAND + LP_MAX_TOP];
+    __shared__ uint32_t limit[2];
+    __shared__ int count[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r = blockIdx.x;
+    const T *x = static_cast<const T *>(a.x) + r * a.stride;
+    // head elements up to a multiple of 16 bytes, pieces, tail
+    const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
+    const int head = min(off ? V - off : 0, a.C), pieces = (a.C - head) / V, tail = a.C - head - pieces * V;
+    const T *body = x + head;
+
+    float m = -INFINITY, ref = 0.f, z = 0.f, e = 0.f;
+    auto add = [&](float v) {
+        const float d = v - ref, p = __builtin_amdgcn_exp2f(d * 1.44269504088896f);
+        z += p;
+        e = fmaf(p, fmaxf(d, -200.f), e);                       // (p is 0 from -104 on)
+    };
+    auto raise = [&](float mx) {                                // a new maximum: the sums so far in its units
+        if (mx > m) {
+            const float s = m == -INFINITY ? 0.f : m - mx, f = __builtin_amdgcn_exp2f(s * 1.44269504088896f);
+            e = f == 0.f ? 0.f : f * fmaf(s, z, e);
+            z *= f;
+            m = ref = mx;
+        }
+    };
+    int i = tid;
+    for (; i + (U - 1) * B < pieces; i += U * B) {
+        float v[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) lp_load<DT, V>(body + (int64_t)(i + u * B) * V, v[u]);
+        float mx = v[0][0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) mx = fmaxf(mx, v[u][j]);
+        raise(mx);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) add(v[u][j]);
+    }
+    for (; i < pieces; i += B) {
+        float v[V];
+        lp_load<DT, V>(body + (int64_t)i * V, v);
+        float mx = v[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) mx = fmaxf(mx, v[j]);
+        raise(mx);
+#pragma unroll
+        for (int j = 0; j < V; ++j) add(v[j]);
+    }
+    if (tid < head) { const float v = (float)x[tid]; raise(v); add(v); }
+    if (tid < tail) { const float v = (float)body[pieces * V + tid]; raise(v); add(v); }
+    const float mine = m;
+    // ---- the row's maximum and sums
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    for (int w = 0; w < W; ++w) m = fmaxf(m, red[0][w]);
+    {
+        const float s = mine == -INFINITY ? 0.f : mine - m, f = __builtin_amdgcn_exp2f(s * 1.44269504088896f);
+        e = f == 0.f && z == z ? 0.f : f * fmaf(s, z, e);       // (a NaN sum stays one)
+        z *= f;
+    }
+    for (int o = 32; o >= 1; o >>= 1) { z += __shfl_xor(z, o, 64); e += __shfl_xor(e, o, 64); }
+    if (lane == 0) { red[1][wave] = z; red[2][wave] = e; }
+    if (a.top > 0) maxima[tid] = lp_key(mine);                  // (-inf where a thread has nothing: never among the k best of a larger set)
+    if (tid < 2) count[tid] = 0;
+    __syncthreads();
+    z = red[1][0];
+    e = red[2][0];
+    for (int w = 1; w < W; ++w) { z += red[1][w]; e += red[2][w]; }
+    const float base = m == -INFINITY ? 0.f : m;
+    const bool none = z == 0.f, odd = !(z <= 3.402823466e38f);
+    const float logz = __builtin_amdgcn_logf(z) * 0.693147180559945f;
+    if (tid == 0) a.entropy[r] = none ? 0.f : logz - e / z;
+    lp_given(a, r, tid, B, base, logz, none);
+    const int k = a.top;
+    if (k == 0) return;
+    auto put = [&](int at, unsigned long long c) {
+        a.top_logprob[r * k + at] = none ? -INFINITY : (lp_value((uint32_t)(c >> 32)) - base) - logz;
+        a.top_index[r * k + at] = (int32_t)~(uint32_t)c;
+    };
+    bool done = false;
+    if (!odd) {
+        // ---- T: the largest number (or near it) that at least k threads' maxima reach
+        if (wave == 0) {
+            uint32_t mk[W], lo = ~0u;
+#pragma unroll
+            for (int w = 0; w < W; ++w) { mk[w] = maxima[w * 64 + lane]; lo = min(lo, mk[w]); }
+            for (int o = 32; o >= 1; o >>= 1) lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
+            uint32_t hi = lp_key(m) + 1;                        // reached by nobody; lo by all B >= k
+            lo = __builtin_amdgcn_readfirstlane(lo);
+            hi = __builtin_amdgcn_readfirstlane(hi);
+            int n_lo = B;
+            while (hi - lo > 1 && n_lo > k + LP_SLACK) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                int n = 0;
+#pragma unroll
+                for (int w = 0; w < W; ++w) n += __popcll(__ballot(mk[w] >= mid));
+                if (n >= k) { lo = mid; n_lo = n; } else hi = mid;
+            }
+            if (lane == 0) { limit[0] = lo; limit[1] = n_lo > k + LP_SLACK; }
+        }
+        __syncthreads();
+        const uint32_t T0 = limit[0];
+        const bool ties = limit[1] != 0;                        // then T0 is exactly the k-th largest maximum, and many threads have it
+        const uint32_t from = ties ? T0 + 1 : T0;
+        if (maxima[tid] >= from) picked[atomicAdd(&count[0], 1)] = tid;
+        __syncthreads();
+        const int n_picked = count[0], per = (pieces + B - 1) / B;
+        auto keep = [&](float v, int c) {
+            const uint32_t key = lp_key(v);
+            if (key >= from) {
+                const int at = atomicAdd(&count[1], 1);
+                if (at < LP_CAND) cand[at] = (unsigned long long)key << 32 | (uint32_t)~c;
+            }
+        };
+        for (int64_t j = tid; j < (int64_t)n_picked * per; j += B) {
+            const int piece = (int)(j % per) * B + (int)picked[j / per];
+            if (piece < pieces) {
+                float v[V];
+                lp_load<DT, V>(body + (int64_t)piece * V, v);
+#pragma unroll
+                for (int q = 0; q < V; ++q) keep(v[q], head + piece * V + q);
+            }
+        }
+        for (int j = tid; j < n_picked; j += B) {
+            const int t = (int)picked[j];
+            if (t < head) keep((float)x[t], t);
+            if (t < tail) keep((float)body[pieces * V + t], head + pieces * V + t);
+        }
+        __syncthreads();
+        int n = count[1];
+        bool fits = n <= LP_CAND;
+        if (ties && n < k) {                                    // the lowest classes equal to T0 make up the rest
+            __syncthreads();
+            for (int c0 = 0; c0 < a.C && n < k; c0 += B) {
+                const int c = c0 + tid;
+                if (c < a.C && lp_key((float)x[c]) == T0) cand[atomicAdd(&count[1], 1)] = (unsigned long long)T0 << 32 | (uint32_t)~c;
+                __syncthreads();
+                n = count[1];                                   // (at most k - 1 + B)
+                __syncthreads();
+            }
+        }
+        if (fits) {
+            for (int j = tid; j < n; j += B) {
+                const unsigned long long c = cand[j];
+                int rank = 0;
+                for (int q = 0; q < n; ++q) rank += cand[q] > c;
+                if (rank < k) put(rank, c);
+            }
+            done = true;
+        }
+    }
+    if (done) return;
+    unsigned long long last = ~0ull;                            // (key, ~class) of the previous alternative
+    for (int t = 0; t < k; ++t) {
         unsigned long long b = 0;
-        for (int c = tid; c < a.C; c += 256) {
-            const unsigned long long k = (unsigned long long)lp_key((float)x[c]) << 32 | (uint32_t)~c;
-            if ((i == 0 || k < last) && k > b) b = k;
+        for (int c = tid; c < a.C; c += B) {
+            const unsigned long long q = (unsigned long long)lp_key((float)x[c]) << 32 | (uint32_t)~c;
+            if ((t == 0 || q < last) && q > b) b = q;
         }
-        for (int off = 32; off >= 1; off >>= 1) { const unsigned long long o = __shfl_xor(b, off, 64); b = o > b ? o : b; }
+        for (int o = 32; o >= 1; o >>= 1) { const unsigned long long q = __shfl_xor(b, o, 64); b = q > b ? q : b; }
         __syncthreads();
-        if (lane == 0) best[wave] = b;
+        if (lane == 0) cand[wave] = b;
         __syncthreads();
-        for (int w = 0; w < 4; ++w) b = best[w] > b ? best[w] : b;
+        for (int w = 0; w < W; ++w) b = cand[w] > b ? cand[w] : b;
         last = b;
-        if (tid == 0) {
-            a.top_logprob[r * a.top + i] = logp(lp_value((uint32_t)(b >> 32)));
-            a.top_index[r * a.top + i] = (int32_t)~(uint32_t)b;
-        }
+        if (tid == 0) put(t, b);
     }
 }
 

@@ -501,7 +501,7 @@ def _check_scores(x, tokens, top, got):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("classes", [1, 2, 3, 63, 64, 65, 232, 1000, 1025, 4099, 33001])
+@pytest.mark.parametrize("classes", [1, 2, 3, 63, 64, 65, 232, 256, 257, 511, 513, 1000, 1025, 4096, 4099, 33001, 70007])
 def test_gpu_logprobs_sizes(classes, kind):
     rows = 5 if classes > 2000 else 13
     g = _gen(classes)
@@ -514,7 +514,7 @@ def test_gpu_logprobs_sizes(classes, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("classes", [40, 700, 9000])
+@pytest.mark.parametrize("classes", [40, 300, 700, 9000, 40000])
 def test_gpu_logprobs_special_rows(classes):
     """ties, masks of -inf and of the lowest number, rows without anything, NaN and infinities, numbers at the ends of the range"""
     low = torch.finfo(torch.float32).min
