@@ -103,6 +103,9 @@ template <int DT, int FMT> int read_by_dim(dim3 (*grid)(uint32_t, int), int D, v
 
 dim3 row_grid(uint32_t rows, int D) { const uint32_t per = 256 / (D / 8); return dim3((rows + per - 1) / per); }
 
+// 32 rows a wave where their queries and sums leave room for two waves in a SIMD's registers
+constexpr bool two_tiles(int dtype, int D) { return D <= 64 || (D == 128 && dtype != POCR_F32); }
+
 // How the work of one attention call is cut.
 struct AttendPlan { int rt, tiles, nsplit, waves; int64_t groups; };
 
@@ -110,11 +113,11 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     AttendPlan p;
     const int64_t most = t->max_queries > 0 && t->max_queries < t->tokens ? t->max_queries : t->tokens;
     const int64_t rows = most * (t->heads / c->kv_heads), pairs = (int64_t)t->seqs * c->kv_heads;
-    p.rt = rows > 16 && c->head_dim <= 128 ? 2 : 1;
+    p.rt = rows > 16 && two_tiles(t->dtype, c->head_dim) ? 2 : 1;
     p.tiles = (int)std::min<int64_t>((rows + 16 * p.rt - 1) / (16 * p.rt), 1024);
     const int64_t units = pairs * p.tiles, blocks = (((int64_t)t->max_pages << page_shift(c)) + 31) / 32;
     const int64_t want = (512 + units - 1) / units, most_splits = std::max<int64_t>(1, blocks / 8);
-    p.nsplit = (int)std::min<int64_t>(std::min(want, most_splits), 128);
+    p.nsplit = (int)std::min<int64_t>(std::min(want, most_splits), TA_MAX_SPLITS);
     p.waves = units >= 2048 ? 1 : TA_WAVES;
     p.groups = (pairs * p.nsplit + 7) / 8 * 8 * p.tiles;
     return p;
@@ -123,7 +126,7 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
 template <int DT, int FMT, int D> int attend(const AttendPlan &p, void *stream, const TreeAttnArgs &a) {
     const char *w = "pocr_tree_attention";
     const dim3 grid((unsigned)p.groups), block(64 * p.waves);
-    constexpr int RT = D <= 128 ? 2 : 1;
+    constexpr int RT = two_tiles(DT, D) ? 2 : 1;
     const int rc = p.rt == 1 ? launch(w, tree_attention_kernel<DT, FMT, D, 1>, grid, block, stream, a) : launch(w, tree_attention_kernel<DT, FMT, D, RT>, grid, block, stream, a);
     if (rc || p.nsplit == 1) return rc;
     return launch(w, tree_attention_join_kernel<DT, D>, dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), stream, a);

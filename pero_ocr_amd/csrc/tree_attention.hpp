@@ -47,34 +47,35 @@ struct TreeAttnArgs {
     float scale;
 };
 
-struct TreeSeq { int64_t first; int32_t n; int64_t len; };
+// arrays that no kernel of the call writes, read by a whole wave at one place: through the scalar cache
+typedef const __attribute__((address_space(4))) int32_t *ScalarInts;
+
+struct TreeSeq { int32_t first, n, len; };          // (positions and rows are 32-bit numbers: lengths and q_start are)
 
 __device__ __forceinline__ TreeSeq tree_seq(const TreeAttnArgs &a, int s) {
-    const int64_t b = a.starts[s], e = a.starts[s + 1];
+    const ScalarInts starts = (ScalarInts)a.starts, lengths = (ScalarInts)a.lengths;
+    const int32_t b = starts[s], e = starts[s + 1], total = (int32_t)a.tokens, l = lengths[s];
     TreeSeq r;
-    r.first = b < 0 ? 0 : (b > a.tokens ? a.tokens : b);
-    const int64_t end = e > a.tokens ? a.tokens : e;
-    r.n = (int32_t)(end > r.first ? end - r.first : 0);
-    const int64_t cap = (int64_t)a.max_pages << a.page_shift, l = a.lengths[s];
-    r.len = l < 0 ? 0 : (l > cap ? cap : l);
+    r.first = min(max(b, 0), total);
+    r.n = max(min(e, total) - r.first, 0);
+    const int64_t cap = (int64_t)a.max_pages << a.page_shift;
+    r.len = (int32_t)min((int64_t)max(l, 0), cap);
     return r;
 }
 
 // low `n` bits of a word, n of any size
-__device__ __forceinline__ uint32_t low_bits(int64_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t low_bits(int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
 // which of the 32 drafted tokens d0 .. d0 + 31 new token i sees; d < 0: an older position, seen by all
-__device__ __forceinline__ uint32_t tree_window(const uint64_t *row, int32_t words, int32_t i, int64_t d0) {
-    if (d0 + 31 < 0) return ~0u;
+__device__ __forceinline__ uint32_t tree_window(const uint64_t *row, int32_t words, int32_t i, int32_t d0) {
+    if (d0 < -31) return ~0u;
     if (!row) return low_bits(i - d0 + 1);
-    const int64_t f = d0 < 0 ? 0 : d0;
-    const int64_t w = f >> 6;
-    const int sh = (int)(f & 63);
+    const int32_t f = max(d0, 0), w = f >> 6, sh = f & 63;
     uint64_t lo = w < words ? row[w] : 0;
     lo >>= sh;
     if (sh && w + 1 < words) lo |= row[w + 1] << (64 - sh);
     const uint32_t bits = (uint32_t)lo;
-    return d0 < 0 ? (bits << (int)-d0) | low_bits(-d0) : bits;
+    return d0 < 0 ? (bits << -d0) | low_bits(-d0) : bits;
 }
 
 __device__ __forceinline__ float row_max(float x) {          // over the four lanes of a row
@@ -137,7 +138,7 @@ template <int FMT, int D> struct KvBlock {
     uint32_t ke[2], ve[2];
 
     // base[h]: row number of key 0 of half h (of row 0 where the page is absent: in bounds, and masked by the caller)
-    __device__ __forceinline__ void load(const TreeAttnArgs &a, const int64_t (&base)[2], int lane) {
+    __device__ __forceinline__ void load_keys(const TreeAttnArgs &a, const int64_t (&base)[2], int lane) {
         const int i = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -150,6 +151,9 @@ template <int FMT, int D> struct KvBlock {
             }
             if constexpr (FMT == KV_FP8) ke[h] = a.k_exp[base[h] + i];
         }
+    }
+    __device__ __forceinline__ void load_values(const TreeAttnArgs &a, const int64_t (&base)[2], int lane) {
+        const int i = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint8_t *vr = static_cast<const uint8_t *>(a.v) + (base[h] + 4 * g) * (D * ES) + i * VB;
@@ -233,7 +237,7 @@ template <int FMT> __device__ __forceinline__ float kv_element(const void *data,
 constexpr int TA_WAVES = 4;            // waves of a workgroup: they take the key blocks in turn
 
 template <int DT, int FMT, int D, int RT>
-__global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnArgs a) {
+__global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attention_kernel(TreeAttnArgs a) {
     using T = typename ElemOf<DT>::type;
     using Block = KvBlock<FMT, D>;
     constexpr int QP = DT == DT_F32 ? 3 : DT == DT_F16 ? 2 : 1;      // planes of the query
@@ -253,35 +257,37 @@ __global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnA
     const int split = (int)(stream / pairs), pair = (int)(stream - split * pairs), s = pair / a.kv_heads, hk = pair - s * a.kv_heads;
     const TreeSeq sq = tree_seq(a, s);
     const int group = a.heads / a.kv_heads;
-    const int64_t rows = (int64_t)sq.n * group;
+    const uint32_t rows = (uint32_t)sq.n * (uint32_t)group;           // (tokens * heads < 2^31)
     const int32_t *table = a.table + s * a.table_stride;
+    // scores in units of log2: the sign of the scale goes to the query, so that the largest product is the largest score; 0 makes the query 0
     const float c = a.scale * 1.44269504088896f;
-    const float csign = c < 0.f ? -1.f : 1.f, cabs = fabsf(c);
+    const float csign = c == 0.f ? 0.f : c < 0.f ? -1.f : 1.f, cabs = c == 0.f ? 1.f : fabsf(c);
 
     if (a.zero_rest && s == a.seqs - 1 && split == 0) {               // rows of no sequence
-        const int64_t rest = (a.tokens - sq.first - sq.n) * group;
-        for (int64_t r = tile0 * (int64_t)blockDim.x + tid; r < rest; r += (int64_t)a.tiles * blockDim.x) {
-            const int64_t at = (sq.first + sq.n + r / group) * a.heads + hk * group + r % group;
+        const uint32_t rest = ((uint32_t)a.tokens - (uint32_t)(sq.first + sq.n)) * (uint32_t)group;
+        for (uint32_t r = tile0 * blockDim.x + tid; r < rest; r += (uint32_t)a.tiles * blockDim.x) {
+            const int64_t at = (int64_t)(sq.first + sq.n + (int32_t)(r / group)) * a.heads + hk * group + (int32_t)(r % group);
+#pragma unroll 1
             for (int d = 0; d < D; ++d) static_cast<T *>(a.out)[at * D + d] = (T)0.f;
             if (a.lse) a.lse[at] = -INFINITY;
         }
     }
 
-    const int64_t blocks = (sq.len + 31) >> 5, per = (blocks + a.nsplit - 1) / a.nsplit;
-    const int64_t first_block = split * per, end_block = first_block + per < blocks ? first_block + per : blocks;
-    const int64_t ctx = sq.len - sq.n;
+    const int32_t blocks = (int32_t)(((uint32_t)sq.len + 31u) >> 5), per = (int32_t)(((uint32_t)blocks + a.nsplit - 1u) / (uint32_t)a.nsplit);
+    const int32_t first_block = min(split * per, blocks), end_block = min(first_block + per, blocks);
+    const int32_t ctx = sq.len - sq.n;
 
-    for (int64_t r0 = (int64_t)tile0 * (16 * RT); r0 < rows; r0 += (int64_t)a.tiles * (16 * RT)) {
+    for (uint32_t r0 = tile0 * (16 * RT); r0 < rows; r0 += (uint32_t)a.tiles * (16 * RT)) {
         int32_t tok[RT];
         int64_t at[RT];                                               // row of out, -1: none
         Frag q[RT][ST][QP];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int64_t r = r0 + 16 * rt + row, rr = r < rows ? r : rows - 1;
-            tok[rt] = (int32_t)(rr / group);
-            const int head = hk * group + (int)(rr - (int64_t)tok[rt] * group);
-            at[rt] = r < rows ? (sq.first + tok[rt]) * a.heads + head : -1;
-            const T *qr = static_cast<const T *>(a.q) + (sq.first + tok[rt]) * a.q_ts + head * a.q_hs;
+            const uint32_t r = r0 + 16 * rt + row, rr = min(r, rows - 1);
+            tok[rt] = (int32_t)(rr / (uint32_t)group);
+            const int head = hk * group + (int)(rr - (uint32_t)tok[rt] * (uint32_t)group);
+            at[rt] = r < rows ? (int64_t)(sq.first + tok[rt]) * a.heads + head : -1;
+            const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + head * a.q_hs;
 #pragma unroll
             for (int st = 0; st < ST; ++st) {
                 float x[8];
@@ -302,38 +308,56 @@ __global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnA
 #pragma unroll
             for (int t = 0; t < NB; ++t) o[rt][t] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
         }
-            for (int64_t b = first_block + wave; b < end_block; b += nw) {
-                const int64_t key0 = b << 5;
-                int64_t base[2];
-                uint32_t there = low_bits(sq.len - key0);             // keys that exist at all
+        // a block's keys are requested as soon as the registers of the last one's are free, behind its scores, and its values behind its sums
+        const ScalarInts pages = (ScalarInts)table;
+        auto place = [&](int32_t b, int64_t (&base)[2], uint32_t &there) {
+            const int32_t key0 = b << 5;
+            there = low_bits(sq.len - key0);                          // keys that exist at all
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    base[h] = key0 + 16 * h < sq.len ? kv_row_base(table, a.max_pages, a.num_pages, a.kv_heads, hk, a.page_shift, key0 + 16 * h) : -1;
-                    if (base[h] < 0) {
-                        there &= h ? 0x0000ffffu : 0xffff0000u;
-                        base[h] = 0;
-                    }
-                }
-                Block kv;
-                kv.load(a, base, lane);
+            for (int h = 0; h < 2; ++h) {
+                const int32_t key = key0 + 16 * h;
+                base[h] = 0;
+                const int32_t page = key < sq.len ? pages[key >> a.page_shift] : -1;          // (len <= max_pages * page_size)
+                if (page >= 0 && page < a.num_pages) base[h] = (((int64_t)page * a.kv_heads + hk) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+                else there &= h ? 0x0000ffffu : 0xffff0000u;
+            }
+        };
+        Block kv;
+        int64_t base[2];
+        uint32_t there = 0;
+        if (first_block + wave < end_block) {
+            place(first_block + wave, base, there);
+            kv.load_keys(a, base, lane);
+            kv.load_values(a, base, lane);
+        }
+        for (int32_t b = first_block + wave; b < end_block; b += nw) {
+                const int32_t key0 = b << 5;
+                int64_t next[2];
+                uint32_t next_there = 0;
+                const bool more = b + nw < end_block;
+                if (more) place(b + nw, next, next_there);
                 const bool edge = there != ~0u || key0 + 31 >= ctx;   // some key is not seen by every row
-                if (there != ~0u) kv.drop_values(there, g);
+                ta_f32x4 sc[RT][2];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int st = 0; st < ST; ++st) {
+                        const Frag kf = kv.key(h, st);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int pl = QP - 1; pl >= 0; --pl) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.b, q[rt][st][pl].b, sc[rt][h], 0, 0, 0);
+                    }
+                if (more) kv.load_keys(a, next, lane);
                 float p[RT][8];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    ta_f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int st = 0; st < ST; ++st) {
-                            const Frag kf = kv.key(h, st);
-#pragma unroll
-                            for (int pl = QP - 1; pl >= 0; --pl) sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.b, q[rt][st][pl].b, sc[h], 0, 0, 0);
-                        }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) p[rt][j] = sc[j >> 2][j & 3];
+                    for (int j = 0; j < 8; ++j) p[rt][j] = sc[rt][j >> 2][j & 3];
                     if (edge) {
-                        const uint32_t vis = there & tree_window(a.mask ? a.mask + (sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], key0 - ctx);
+                        const uint32_t vis = there & tree_window(a.mask ? a.mask + (int64_t)(sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], key0 - ctx);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) p[rt][j] = vis >> ((j >> 2) * 16 + 4 * g + (j & 3)) & 1 ? p[rt][j] : -INFINITY;
                     }
@@ -348,10 +372,11 @@ __global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnA
                         for (int t = 0; t < NB; ++t) o[rt][t] *= alpha;
                         m[rt] = mx;
                     }
+                    // (2^-inf is 0; without a maximum yet the reference is 0)
                     const float mc = m[rt] == -INFINITY ? 0.f : m[rt] * cabs;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        p[rt][j] = p[rt][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(p[rt][j], cabs, -mc));
+                        p[rt][j] = __builtin_amdgcn_exp2f(fmaf(p[rt][j], cabs, -mc));
                         l[rt] += p[rt][j];
                     }
                     if constexpr (FMT == KV_FP8) {
@@ -359,6 +384,7 @@ __global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnA
                         for (int j = 0; j < 8; ++j) p[rt][j] *= kv_scale((uint8_t)(kv.ve[j >> 2] >> (8 * (j & 3))));
                     }
                 }
+                if (there != ~0u) kv.drop_values(there, g);
                 Frag pf[RT][PP];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) split_planes<PP>(p[rt], pf[rt]);
@@ -374,7 +400,11 @@ __global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnA
                             for (int pl = PP - 1; pl >= 0; --pl)
                                 o[rt][w * TW + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[t].b, pf[rt][pl].b, o[rt][w * TW + t], 0, 0, 0);
                 }
-            }
+                if (more) kv.load_values(a, next, lane);
+                base[0] = next[0];
+                base[1] = next[1];
+                there = next_there;
+        }
         bool odd = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -389,21 +419,21 @@ __global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnA
                 l[rt] = 0.f;
 #pragma unroll
                 for (int t = 0; t < NB; ++t) o[rt][t] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
-                const int64_t r = r0 + 16 * rt + row, rr = r < rows ? r : rows - 1;
-                const T *qr = static_cast<const T *>(a.q) + (sq.first + tok[rt]) * a.q_ts + (hk * group + (rr - (int64_t)tok[rt] * group)) * a.q_hs;
-                for (int64_t b = first_block + wave; b < end_block; b += nw)
-                    for (int64_t key = b << 5; key < (b + 1) << 5 && key < sq.len; ++key) {
+                const uint32_t rr = min(r0 + 16 * rt + row, rows - 1);
+                const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + (hk * group + (int)(rr - (uint32_t)tok[rt] * (uint32_t)group)) * a.q_hs;
+                for (int32_t b = first_block + wave; b < end_block; b += nw)
+                    for (int32_t key = b << 5, n = min(32, sq.len - key); n > 0; --n, ++key) {
                         const int64_t kr = kv_row_base(table, a.max_pages, a.num_pages, a.kv_heads, hk, a.page_shift, key);
                         if (kr < 0) continue;                         // (the same for all lanes)
                         float dot = 0.f;
 #pragma unroll 1
                         for (int d = g * (D / 4); d < (g + 1) * (D / 4); ++d) dot += (float)qr[d] * csign * kv_element<FMT>(a.k, a.k_exp, kr, D, d);
                         dot = row_sum(dot);
-                        const bool sees = tree_window(a.mask ? a.mask + (sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], key - ctx) & 1;
+                        const bool sees = tree_window(a.mask ? a.mask + (int64_t)(sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], key - ctx) & 1;
                         if (!sees) continue;
                         const float mx = fmaxf(m[rt], dot);
                         const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[rt] - mx) * cabs);
-                        const float mc = mx == -INFINITY ? 0.f : mx * cabs, p = dot == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(dot, cabs, -mc));
+                        const float mc = mx == -INFINITY ? 0.f : mx * cabs, p = __builtin_amdgcn_exp2f(fmaf(dot, cabs, -mc));
                         m[rt] = mx;
                         l[rt] = l[rt] * alpha + (g == 0 ? p : 0.f);
 #pragma unroll
@@ -489,30 +519,47 @@ __global__ __launch_bounds__(64 * TA_WAVES) void tree_attention_kernel(TreeAttnA
 }
 
 // The splits' sums of one row meet: a wave per (token, head) of a sequence.  Rows of no sequence are left to the kernel above.
+constexpr int TA_MAX_SPLITS = 128;
+
 template <int DT, int D>
 __global__ __launch_bounds__(256) void tree_attention_join_kernel(TreeAttnArgs a) {
     using T = typename ElemOf<DT>::type;
+    constexpr int E = D < 64 ? 1 : D / 64;                            // neighbouring elements of a lane
     const int lane = threadIdx.x & 63;
-    const int64_t total = a.tokens * a.heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t total = (uint32_t)a.tokens * (uint32_t)a.heads, at = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (at >= total) return;
-    const int64_t token = at / a.heads;
-    if (token < a.starts[0] || token >= a.starts[a.seqs]) return;
-    const float *ml = a.part + (int64_t)a.nsplit * total * D + at * 2;
-    float m = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, ml[s * total * 2]);
-    float l = 0.f, o[(D + 63) / 64] = {};
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float ms = ml[s * total * 2];
-        if (ms == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ms - m);
-        l += f * ml[s * total * 2 + 1];
+    const int32_t token = (int32_t)(at / (uint32_t)a.heads);
+    const ScalarInts starts = (ScalarInts)a.starts;
+    if (token < starts[0] || token >= starts[a.seqs]) return;
+    const float *ml = a.part + (int64_t)a.nsplit * total * D + (int64_t)at * 2;
+    float ms[2], ls[2];                                               // splits lane and lane + 64
 #pragma unroll
-        for (int c = 0; c < (D + 63) / 64; ++c)
-            if (lane + 64 * c < D) o[c] += f * a.part[(s * total + at) * D + lane + 64 * c];
+    for (int i = 0; i < 2; ++i) {
+        const int s = lane + 64 * i;
+        ms[i] = s < a.nsplit ? ml[(int64_t)s * total * 2] : -INFINITY;
+        ls[i] = s < a.nsplit ? ml[(int64_t)s * total * 2 + 1] : 0.f;
     }
+    float m = fmaxf(ms[0], ms[1]);
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float f[2], l = 0.f, acc[E] = {};
 #pragma unroll
-    for (int c = 0; c < (D + 63) / 64; ++c)
-        if (lane + 64 * c < D) static_cast<T *>(a.out)[at * D + lane + 64 * c] = (T)(l == 0.f ? 0.f : o[c] / l);
+    for (int i = 0; i < 2; ++i) {
+        f[i] = ms[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[i] - m);
+        l += f[i] * ls[i];
+    }
+    for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
+    const float *po = a.part + (int64_t)at * D + (D < 64 ? lane & (D - 1) : lane * E);
+#pragma unroll 8
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float fs = __shfl(s < 64 ? f[0] : f[1], s & 63, 64);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += fs * po[(int64_t)s * total * D + e];
+    }
+    T *out = static_cast<T *>(a.out) + (int64_t)at * D + lane * E;
+    if (lane * E < D) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) out[e] = (T)(l == 0.f ? 0.f : acc[e] / l);
+    }
     if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147180559945f;
 }
 
