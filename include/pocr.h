@@ -411,7 +411,7 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const 
  * (lse: -inf) with zero_rest.  max_queries: the most new tokens of one sequence, if known (0: unknown): it shapes the launch, any
  * value gives the same answer.  Sums and the softmax are in 32 bits. */
 typedef struct pocr_tree_attention_args {
-    const void *q;                    /* [tokens][heads][head_dim], element strides q_token_stride, q_head_stride */
+    const void *q;                    /* [tokens][heads][head_dim], element strides q_token_stride, q_head_stride; rows start at multiples of 16 bytes */
     void *out;                        /* [tokens][heads][head_dim] contiguous, 16-byte aligned */
     float *lse;                       /* [tokens][heads] log of the sum of exp, or NULL */
     const int32_t *page_table, *lengths, *q_start;

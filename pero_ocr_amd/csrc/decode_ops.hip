@@ -116,9 +116,12 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     p.rt = rows > 16 && two_tiles(t->dtype, c->head_dim) ? 2 : 1;
     p.tiles = (int)std::min<int64_t>((rows + 16 * p.rt - 1) / (16 * p.rt), 1024);
     const int64_t units = pairs * p.tiles, blocks = (((int64_t)t->max_pages << page_shift(c)) + 31) / 32;
-    const int64_t want = (512 + units - 1) / units, most_splits = std::max<int64_t>(1, blocks / 8);
+    // A workgroup costs about 4 us to start and to end (cold scalar loads, the join of its waves), a block of 32 keys 0.3 us a wave: no split below
+    // 16 blocks (one sequence, 4129 keys, 264 rows: 4 to 8 splits 20-21 us, 16 splits 24 us), and no more workgroups than two rounds
+    // over the chip (four sequences of 60-131 thousand keys: 512 workgroups 188 us, 1024 181 us, 2048 197 us).
+    const int64_t want = (1024 + units - 1) / units, most_splits = std::max<int64_t>(1, blocks / 16);
     p.nsplit = (int)std::min<int64_t>(std::min(want, most_splits), TA_MAX_SPLITS);
-    p.waves = units >= 2048 ? 1 : TA_WAVES;
+    p.waves = p.rt == 1 && units >= 2048 ? 1 : 4;
     p.groups = (pairs * p.nsplit + 7) / 8 * 8 * p.tiles;
     return p;
 }
@@ -127,7 +130,9 @@ template <int DT, int FMT, int D> int attend(const AttendPlan &p, void *stream, 
     const char *w = "pocr_tree_attention";
     const dim3 grid((unsigned)p.groups), block(64 * p.waves);
     constexpr int RT = two_tiles(DT, D) ? 2 : 1;
-    const int rc = p.rt == 1 ? launch(w, tree_attention_kernel<DT, FMT, D, 1>, grid, block, stream, a) : launch(w, tree_attention_kernel<DT, FMT, D, RT>, grid, block, stream, a);
+    const int rc = p.waves == 1 ? launch(w, tree_attention_kernel<DT, FMT, D, 1, 1>, grid, block, stream, a)
+                   : p.rt == 1  ? launch(w, tree_attention_kernel<DT, FMT, D, 1, 4>, grid, block, stream, a)
+                                : launch(w, tree_attention_kernel<DT, FMT, D, RT, 4>, grid, block, stream, a);
     if (rc || p.nsplit == 1) return rc;
     return launch(w, tree_attention_join_kernel<DT, D>, dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), stream, a);
 }
@@ -224,7 +229,8 @@ int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, con
     if (t->tokens == 0) return 0;
     if (!t->q || !t->out || !t->lengths || !t->q_start || (t->max_pages > 0 && !t->page_table)) return refuse("pocr_tree_attention: NULL pointer");
     const int es = elem_size(t->dtype);
-    if (!aligned(t->q, es) || !aligned(t->out, 16) || !aligned(t->lse, 4) || !aligned(t->mask, 8) || !aligned(t->lengths, 4) || !aligned(t->q_start, 4) || !aligned(t->page_table, 4))
+    if (!aligned(t->q, 16) || (t->q_token_stride * es) % 16 || (t->q_head_stride * es) % 16) return refuse("pocr_tree_attention: rows of q must start at multiples of 16 bytes");
+    if (!aligned(t->out, 16) || !aligned(t->lse, 4) || !aligned(t->mask, 8) || !aligned(t->lengths, 4) || !aligned(t->q_start, 4) || !aligned(t->page_table, 4))
         return refuse("pocr_tree_attention: a pointer is not aligned to its element (out: to 16 bytes)");
     const AttendPlan p = attend_plan(c, t);
     const int64_t need = p.nsplit == 1 ? 0 : (int64_t)p.nsplit * t->tokens * t->heads * (c->head_dim + 2) * 4;
@@ -232,10 +238,9 @@ int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, con
         return refuse("pocr_tree_attention: a workspace of %lld bytes, aligned to 16, is needed (pocr_tree_attention_workspace)", (long long)need);
     OnDevice dev;
     if (dev.enter(device_id)) return 1;
-    const bool q_vec = aligned(t->q, 16) && (t->q_token_stride * es) % 16 == 0 && (t->q_head_stride * es) % 16 == 0;
     TreeAttnArgs a{t->q, c->k, c->v, c->k_exp, c->v_exp, t->page_table, t->lengths, t->q_start, t->mask, t->out, t->lse, static_cast<float *>(t->workspace),
                    t->q_token_stride, t->q_head_stride, t->page_table_stride, t->mask_stride, t->tokens, t->seqs, t->heads, c->kv_heads, c->num_pages, page_shift(c),
-                   t->max_pages, t->mask_words, t->zero_rest, p.nsplit, p.tiles, q_vec, t->scale};
+                   t->max_pages, t->mask_words, t->zero_rest, p.nsplit, p.tiles, t->scale};
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         return c->format == POCR_KV_FP8 ? attend_by_dim<DT, KV_FP8>(c->head_dim, p, stream, a) : attend_by_dim<DT, KV_BF16>(c->head_dim, p, stream, a);

@@ -5,16 +5,16 @@
 // positions up to its own.  With s_j = scale * q . k_j over the seen j:  out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j);
 // a token that sees nothing gets out = 0, lse = -inf.  Query head h reads key head h / (heads / kv_heads).
 //
-// One pass over the keys with a running maximum and sum.  A wave owns RT * 16 rows (a row = one new token and one of the query heads that
+// One pass over the keys with a running reference (a maximum that lags by at most 2^8) and sum.  A wave owns RT * 16 rows (a row = one new token and one of the query heads that
 // share the key head) and takes blocks of 32 keys; both products run on v_mfma_f32_16x16x32_bf16, transposed, so that a row is always
-// lane & 15 and nothing is exchanged between lanes but the row maximum:
+// lane & 15 and nothing is exchanged between lanes but, now and then, the row maximum:
 //   S^T = K Q^T     lane (row, g = lane / 16) gets the scores of keys 4 g + r and 16 + 4 g + r of the block, r = 0..3
 //   O^T = V^T P^T   takes exactly these eight probabilities as its operand when V^T is fed in the same key order
 // Keys and values go from HBM straight into registers, no LDS and no barrier in the loop.  K: a lane holds a quarter of one key's
 // row (which quarter of each 64 elements is free to choose, Q is laid out to match), so whole lines are read.  V: a lane loads D / 16 neighbouring elements
 // of eight keys and transposes them with byte permutes; tile c of the product then is elements c, D/16 + c, 2 D/16 + c, ... and a lane ends up with
 // D / 4 neighbouring outputs of its row.
-// 8-bit codes become bfloat16 exactly, K's by v_cvt_scalef32 with the key's own power of two; V's power of two goes to the probability.
+// 8-bit codes become bfloat16 exactly, by v_cvt_scalef32 with the key's own power of two.
 // What is rounded: the probability enters the second product as bf16 planes (cut, cut, rounded), two for 16-bit queries (2^-17 of it: one plane's 2^-9
 // would add as much error as rounding the result does) and three for float32 (2^-25); a float16 or float32 query is two or three bf16 planes (exact / 2^-25).
 // Scores, statistics and sums are float32.
@@ -43,7 +43,7 @@ struct TreeAttnArgs {
     float *lse;
     float *part;                  // nsplit > 1: sums [nsplit][tokens * heads][D], then (maximum, sum) [nsplit][tokens * heads][2]
     int64_t q_ts, q_hs, table_stride, mask_stride, tokens;
-    int32_t seqs, heads, kv_heads, num_pages, page_shift, max_pages, mask_words, zero_rest, nsplit, tiles, q_vec;
+    int32_t seqs, heads, kv_heads, num_pages, page_shift, max_pages, mask_words, zero_rest, nsplit, tiles;
     float scale;
 };
 
@@ -137,36 +137,37 @@ template <int FMT, int D> struct KvBlock {
     uint32_t v[8][VW];
     uint32_t ke[2], ve[2];
 
-    // base[h]: row number of key 0 of half h (of row 0 where the page is absent: in bounds, and masked by the caller)
-    __device__ __forceinline__ void load_keys(const TreeAttnArgs &a, const int64_t (&base)[2], int lane) {
-        const int i = lane & 15, g = lane >> 4;
+    // base[h]: row number of key 0 of half h (of row 0 where the page is absent: in bounds, and masked by the caller); the same for the whole
+    // wave, so that a lane's part of the address is a constant 32-bit offset
+    __device__ __forceinline__ void load_keys(const TreeAttnArgs &a, const int64_t (&base)[2], uint32_t lane) {
+        const uint32_t i = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint8_t *kr = static_cast<const uint8_t *>(a.k) + (base[h] + i) * (D * ES);
+            const uint8_t *kb = static_cast<const uint8_t *>(a.k) + base[h] * (D * ES);
             if constexpr (KW == 2) {
-                *reinterpret_cast<kv_u32x2 *>(k[h]) = *reinterpret_cast<const kv_u32x2 *>(kr + g * 8);
+                *reinterpret_cast<kv_u32x2 *>(k[h]) = *reinterpret_cast<const kv_u32x2 *>(kb + (i * (D * ES) + g * 8));
             } else {
 #pragma unroll
-                for (int c = 0; c < KW / 4; ++c) *reinterpret_cast<kv_u32x4 *>(k[h] + 4 * c) = *reinterpret_cast<const kv_u32x4 *>(kr + c * 64 + g * 16);
+                for (int c = 0; c < KW / 4; ++c) *reinterpret_cast<kv_u32x4 *>(k[h] + 4 * c) = *reinterpret_cast<const kv_u32x4 *>(kb + (i * (D * ES) + g * 16) + c * 64);
             }
-            if constexpr (FMT == KV_FP8) ke[h] = a.k_exp[base[h] + i];
+            if constexpr (FMT == KV_FP8) ke[h] = (a.k_exp + base[h])[i];
         }
     }
-    __device__ __forceinline__ void load_values(const TreeAttnArgs &a, const int64_t (&base)[2], int lane) {
-        const int i = lane & 15, g = lane >> 4;
+    __device__ __forceinline__ void load_values(const TreeAttnArgs &a, const int64_t (&base)[2], uint32_t lane) {
+        const uint32_t i = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint8_t *vr = static_cast<const uint8_t *>(a.v) + (base[h] + 4 * g) * (D * ES) + i * VB;
+            const uint8_t *vb = static_cast<const uint8_t *>(a.v) + base[h] * (D * ES);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 uint32_t *w = v[4 * h + t];
-                const uint8_t *p = vr + t * (D * ES);
+                const uint8_t *p = vb + (g * (4 * D * ES) + i * VB) + t * (D * ES);
                 if constexpr (VB == 2) w[0] = *reinterpret_cast<const uint16_t *>(p);
                 else if constexpr (VB == 4) w[0] = *reinterpret_cast<const uint32_t *>(p);
                 else if constexpr (VB == 8) *reinterpret_cast<kv_u32x2 *>(w) = *reinterpret_cast<const kv_u32x2 *>(p);
                 else {
 #pragma unroll
-                    for (int c = 0; c < VB / 16; ++c) *reinterpret_cast<kv_u32x4 *>(w + 4 * c) = reinterpret_cast<const kv_u32x4 *>(p)[c];
+                    for (int c = 0; c < VB / 16; ++c) *reinterpret_cast<kv_u32x4 *>(w + 4 * c) = *reinterpret_cast<const kv_u32x4 *>(p + 16 * c);
                 }
             }
             if constexpr (FMT == KV_FP8) ve[h] = *reinterpret_cast<const uint32_t *>(a.v_exp + base[h] + 4 * g);
@@ -191,32 +192,25 @@ template <int FMT, int D> struct KvBlock {
         else if constexpr (D == 32) return g * 8;
         else return (st >> 1) * 64 + g * 16 + (st & 1) * 8;
     }
-    // operands of the second product: NT = min(4 or 2, D / 16) tiles made of dword w of every key
-    static constexpr int TW = FMT == KV_FP8 ? (VB < 4 ? 2 : 4) : 2;
+    // operands of the second product: the TW tiles made of dword w of every key
+    static constexpr int TW = VB < 4 ? 2 : 4 / ES;
     __device__ __forceinline__ void values(int w, Frag (&f)[TW]) const {
-        if constexpr (FMT == KV_FP8) {
+        uint32_t x[8][TW / 2];                                        // neighbouring pairs of every key's elements, in bfloat16
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t w0 = v[4 * h][w], w1 = v[4 * h + 1][w], w2 = v[4 * h + 2][w], w3 = v[4 * h + 3][w];
-                const uint32_t x0 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), y0 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
-                uint32_t t[4];
-                t[0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
-                t[1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
-                if constexpr (TW == 4) {
-                    const uint32_t x1 = __builtin_amdgcn_perm(w1, w0, 0x07030602u), y1 = __builtin_amdgcn_perm(w3, w2, 0x07030602u);
-                    t[2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
-                    t[3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
-                }
+        for (int t = 0; t < 8; ++t) {
+            if constexpr (FMT == KV_FP8) {
+                const float s = kv_scale((uint8_t)(ve[t >> 2] >> (8 * (t & 3))));
+                x[t][0] = fp8_pair(v[t][w], s, false);
+                if constexpr (TW == 4) x[t][1] = fp8_pair(v[t][w], s, true);
+            } else x[t][0] = v[t][w];
+        }
 #pragma unroll
-                for (int c = 0; c < TW; ++c) { f[c].u[2 * h] = fp8_pair(t[c], 1.f, false); f[c].u[2 * h + 1] = fp8_pair(t[c], 1.f, true); }
-            }
-        } else {
+        for (int c = 0; c < TW / 2; ++c)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f[0].u[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], 0x05040100u);
-                f[1].u[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], 0x07060302u);
+                f[2 * c].u[j] = __builtin_amdgcn_perm(x[2 * j + 1][c], x[2 * j][c], 0x05040100u);
+                f[2 * c + 1].u[j] = __builtin_amdgcn_perm(x[2 * j + 1][c], x[2 * j][c], 0x07060302u);
             }
-        }
     }
     // keys of the block that nobody may see: their values must not meet a probability 0 (the memory may hold NaN)
     __device__ __forceinline__ void drop_values(uint32_t there, int g) {
@@ -234,10 +228,9 @@ template <int FMT> __device__ __forceinline__ float kv_element(const void *data,
     else return __builtin_amdgcn_cvt_f32_fp8((int)static_cast<const uint8_t *>(data)[row * dim + d], 0) * kv_scale(exp[row]);
 }
 
-constexpr int TA_WAVES = 4;            // waves of a workgroup: they take the key blocks in turn
-
-template <int DT, int FMT, int D, int RT>
-__global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attention_kernel(TreeAttnArgs a) {
+// NW: waves of a workgroup, which take the key blocks in turn
+template <int DT, int FMT, int D, int RT, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kernel(TreeAttnArgs a) {
     using T = typename ElemOf<DT>::type;
     using Block = KvBlock<FMT, D>;
     constexpr int QP = DT == DT_F32 ? 3 : DT == DT_F16 ? 2 : 1;      // planes of the query
@@ -245,9 +238,10 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
     constexpr int NB = D / 16, ST = D / 32, TW = Block::TW;
     const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nw = blockDim.x >> 6;
-    __shared__ ta_f32x4 osum[TA_WAVES / 2][RT * NB][64];
-    __shared__ float stat[TA_WAVES][RT][16][2];
+    constexpr int PITCH = D + 4;                                      // (16 rows, four words each: all 64 banks)
+    __shared__ float osum[NW][RT * 16][PITCH];
+    __shared__ float stat[NW][RT * 16][2], whole[RT * 16][2];
+    __shared__ int64_t place_of[RT * 16];
 
     // workgroups that read the same keys (the row tiles of one sequence, key head and split) are 8 apart: consecutive workgroups go to
     // different XCDs, so these share an L2
@@ -262,10 +256,11 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
     // scores in units of log2: the sign of the scale goes to the query, so that the largest product is the largest score; 0 makes the query 0
     const float c = a.scale * 1.44269504088896f;
     const float csign = c == 0.f ? 0.f : c < 0.f ? -1.f : 1.f, cabs = c == 0.f ? 1.f : fabsf(c);
+    const uint32_t qkeep = c == 0.f ? 0u : ~0u, qflip = c < 0.f ? 0x80008000u : 0u;          // the same for bfloat16 queries, on the bits
 
     if (a.zero_rest && s == a.seqs - 1 && split == 0) {               // rows of no sequence
         const uint32_t rest = ((uint32_t)a.tokens - (uint32_t)(sq.first + sq.n)) * (uint32_t)group;
-        for (uint32_t r = tile0 * blockDim.x + tid; r < rest; r += (uint32_t)a.tiles * blockDim.x) {
+        for (uint32_t r = tile0 * (64 * NW) + tid; r < rest; r += (uint32_t)a.tiles * (64 * NW)) {
             const int64_t at = (int64_t)(sq.first + sq.n + (int32_t)(r / group)) * a.heads + hk * group + (int32_t)(r % group);
 #pragma unroll 1
             for (int d = 0; d < D; ++d) static_cast<T *>(a.out)[at * D + d] = (T)0.f;
@@ -290,12 +285,17 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
             const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + head * a.q_hs;
 #pragma unroll
             for (int st = 0; st < ST; ++st) {
-                float x[8];
-                if (a.q_vec) load8<DT, true>(qr + Block::key_elem(g, st), x);
-                else load8<DT, false>(qr + Block::key_elem(g, st), x);
+                if constexpr (DT == DT_BF16) {
+                    *reinterpret_cast<kv_u32x4 *>(q[rt][st][0].u) = *reinterpret_cast<const kv_u32x4 *>(qr + Block::key_elem(g, st));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= csign;
-                split_planes<QP>(x, q[rt][st]);
+                    for (int j = 0; j < 4; ++j) q[rt][st][0].u[j] = (q[rt][st][0].u[j] & qkeep) ^ qflip;
+                } else {
+                    float x[8];
+                    load8<DT, true>(qr + Block::key_elem(g, st), x);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] *= csign;
+                    split_planes<QP>(x, q[rt][st]);
+                }
             }
         }
 
@@ -308,42 +308,55 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
 #pragma unroll
             for (int t = 0; t < NB; ++t) o[rt][t] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
         }
-        // a block's keys are requested as soon as the registers of the last one's are free, behind its scores, and its values behind its sums
+        // A block's keys are requested as soon as the registers of the last one's are free, behind its scores, and its values behind its sums;
+        // the page ids of the block after that are on their way meanwhile.
         const ScalarInts pages = (ScalarInts)table;
-        auto place = [&](int32_t b, int64_t (&base)[2], uint32_t &there) {
+        auto page_ids = [&](int32_t b, int32_t (&id)[2]) {            // (a block without keys: any entry of the table)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int32_t key = (int32_t)min(((uint32_t)b << 5) + 16u * h, (uint32_t)sq.len - 1u);
+                id[h] = pages[key >> a.page_shift];                   // (len <= max_pages * page_size)
+            }
+        };
+        auto place = [&](int32_t b, const int32_t (&id)[2], int64_t (&base)[2], uint32_t &there) {
             const int32_t key0 = b << 5;
             there = low_bits(sq.len - key0);                          // keys that exist at all
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int32_t key = key0 + 16 * h;
-                base[h] = 0;
-                const int32_t page = key < sq.len ? pages[key >> a.page_shift] : -1;          // (len <= max_pages * page_size)
-                if (page >= 0 && page < a.num_pages) base[h] = (((int64_t)page * a.kv_heads + hk) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-                else there &= h ? 0x0000ffffu : 0xffff0000u;
+                const bool good = (uint32_t)id[h] < (uint32_t)a.num_pages;
+                const int32_t page = good ? id[h] : 0;
+                base[h] = (((int64_t)page * a.kv_heads + hk) << a.page_shift) + ((key0 + 16 * h) & ((1 << a.page_shift) - 1));
+                if (!good) there &= h ? 0x0000ffffu : 0xffff0000u;
             }
         };
         Block kv;
         int64_t base[2];
+        int32_t ids[2];
         uint32_t there = 0;
         if (first_block + wave < end_block) {
-            place(first_block + wave, base, there);
+            page_ids(first_block + wave, ids);
+            place(first_block + wave, ids, base, there);
             kv.load_keys(a, base, lane);
             kv.load_values(a, base, lane);
+            page_ids(first_block + wave + NW, ids);
         }
-        for (int32_t b = first_block + wave; b < end_block; b += nw) {
+        for (int32_t b = first_block + wave; b < end_block; b += NW) {
                 const int32_t key0 = b << 5;
                 int64_t next[2];
                 uint32_t next_there = 0;
-                const bool more = b + nw < end_block;
-                if (more) place(b + nw, next, next_there);
+                const bool more = b + NW < end_block;
+                if (more) {
+                    place(b + NW, ids, next, next_there);
+                    page_ids(b + 2 * NW, ids);
+                }
                 const bool edge = there != ~0u || key0 + 31 >= ctx;   // some key is not seen by every row
                 ta_f32x4 sc[RT][2];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int st = 0; st < ST; ++st)
 #pragma unroll
-                    for (int st = 0; st < ST; ++st) {
+                    for (int h = 0; h < 2; ++h) {
                         const Frag kf = kv.key(h, st);
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
@@ -357,31 +370,30 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
 #pragma unroll
                     for (int j = 0; j < 8; ++j) p[rt][j] = sc[rt][j >> 2][j & 3];
                     if (edge) {
-                        const uint32_t vis = there & tree_window(a.mask ? a.mask + (int64_t)(sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], key0 - ctx);
+                        int32_t d0 = key0 - ctx;
+                        asm volatile("" : "+s"(d0));                  // (nothing of this is worth computing ahead)
+                        const uint32_t vis = there & tree_window(a.mask ? a.mask + (int64_t)(sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], d0);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) p[rt][j] = vis >> ((j >> 2) * 16 + 4 * g + (j & 3)) & 1 ? p[rt][j] : -INFINITY;
                     }
                     float mx = p[rt][0];
 #pragma unroll
                     for (int j = 1; j < 8; ++j) mx = fmaxf(mx, p[rt][j]);
-                    mx = fmaxf(m[rt], row_max(mx));
-                    if (__ballot(mx > m[rt])) {
+                    // the reference moves only when a score passes it by more than 2^8: the sums hold that, and the lanes need not meet otherwise
+                    if (__ballot((mx - m[rt]) * cabs > 8.f)) {
+                        mx = fmaxf(m[rt], row_max(mx));
                         const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[rt] - mx) * cabs);
                         l[rt] *= alpha;
 #pragma unroll
                         for (int t = 0; t < NB; ++t) o[rt][t] *= alpha;
                         m[rt] = mx;
                     }
-                    // (2^-inf is 0; without a maximum yet the reference is 0)
+                    // (2^-inf is 0; without a reference yet it is 0)
                     const float mc = m[rt] == -INFINITY ? 0.f : m[rt] * cabs;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         p[rt][j] = __builtin_amdgcn_exp2f(fmaf(p[rt][j], cabs, -mc));
                         l[rt] += p[rt][j];
-                    }
-                    if constexpr (FMT == KV_FP8) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) p[rt][j] *= kv_scale((uint8_t)(kv.ve[j >> 2] >> (8 * (j & 3))));
                     }
                 }
                 if (there != ~0u) kv.drop_values(there, g);
@@ -405,14 +417,14 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
                 base[1] = next[1];
                 there = next_there;
         }
-        bool odd = false;
+        float odd = 0.f;                                              // NaN if a sum is not finite
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int t = 0; t < NB; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) odd |= !(fabsf(o[rt][t][r]) <= 3.402823466e38f);
-        if (__ballot(odd)) {                                          // key by key, each row only with what it sees
+                for (int r = 0; r < 4; ++r) odd = fmaf(o[rt][t][r], 0.f, odd);
+        if (__ballot(odd != odd)) {                                          // key by key, each row only with what it sees
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 m[rt] = -INFINITY;
@@ -421,7 +433,7 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
                 for (int t = 0; t < NB; ++t) o[rt][t] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
                 const uint32_t rr = min(r0 + 16 * rt + row, rows - 1);
                 const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + (hk * group + (int)(rr - (uint32_t)tok[rt] * (uint32_t)group)) * a.q_hs;
-                for (int32_t b = first_block + wave; b < end_block; b += nw)
+                for (int32_t b = first_block + wave; b < end_block; b += NW)
                     for (int32_t key = b << 5, n = min(32, sq.len - key); n > 0; --n, ++key) {
                         const int64_t kr = kv_row_base(table, a.max_pages, a.num_pages, a.kv_heads, hk, a.page_shift, key);
                         if (kr < 0) continue;                         // (the same for all lanes)
@@ -446,73 +458,65 @@ __global__ __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) void tree_attentio
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) l[rt] = row_sum(l[rt]);
-        // ---- the waves' sums meet: one maximum, then halves add in a fixed order
-        if (nw > 1) {
-            __syncthreads();
-            if (g == 0) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) { stat[wave][rt][row][0] = m[rt]; stat[wave][rt][row][1] = l[rt]; }
-            }
-            __syncthreads();
+        // ---- the waves' sums meet in LDS: one maximum per row, then every thread adds its share of the outputs in a fixed order and writes it
+        // in whole lines
+        __syncthreads();                                              // (the last rows' sums have been read)
+        if (g == 0) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                float mm = stat[0][rt][row][0];
-                for (int w = 1; w < nw; ++w) mm = fmaxf(mm, stat[w][rt][row][0]);
-                float ll = 0.f;
-                for (int w = 0; w < nw; ++w) {
-                    const float mw = stat[w][rt][row][0];
-                    ll += stat[w][rt][row][1] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mw - mm) * cabs));      // (no maximum: 0 or NaN)
-                }
-                const float f = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[rt] - mm) * cabs);
-                if (m[rt] != -INFINITY && f != 1.f) {
-#pragma unroll
-                    for (int t = 0; t < NB; ++t) o[rt][t] *= f;
-                }
-                m[rt] = mm;
-                l[rt] = ll;
-            }
-            for (int half = nw >> 1; half >= 1; half >>= 1) {
-                if (wave >= half && wave < 2 * half) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int t = 0; t < NB; ++t) osum[wave - half][rt * NB + t][lane] = o[rt][t];
-                }
-                __syncthreads();
-                if (wave < half) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int t = 0; t < NB; ++t) o[rt][t] += osum[wave][rt * NB + t][lane];
-                }
-                __syncthreads();
+                stat[wave][16 * rt + row][0] = m[rt];
+                stat[wave][16 * rt + row][1] = l[rt];
+                if (wave == 0) place_of[16 * rt + row] = at[rt];
             }
         }
-        if (wave == 0) {
+        __syncthreads();
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if (at[rt] < 0) continue;
-                const float mc = m[rt] == -INFINITY ? 0.f : m[rt] * cabs;
-                if (a.nsplit > 1) {
-                    float *po = a.part + ((int64_t)split * a.tokens * a.heads + at[rt]) * D + g * (D / 4);
+        for (int rt = 0; rt < RT; ++rt) {
+            float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+            for (int w = 0; w < NW; ++w) mm = fmaxf(mm, stat[w][16 * rt + row][0]);
 #pragma unroll
-                        for (int t = 0; t < NB; t += 2) *reinterpret_cast<kv_f32x2 *>(po + r * NB + t) = (kv_f32x2){o[rt][t][r], o[rt][t + 1][r]};
-                    if (g == 0) {
-                        float *ml = a.part + (int64_t)a.nsplit * a.tokens * a.heads * D + ((int64_t)split * a.tokens * a.heads + at[rt]) * 2;
-                        ml[0] = l[rt] == 0.f ? -INFINITY : mc;        // (in units of log2)
-                        ml[1] = l[rt];
-                    }
-                } else {
-                    const float inv = l[rt] == 0.f ? 0.f : 1.f / l[rt];
-                    T *po = static_cast<T *>(a.out) + at[rt] * D + g * (D / 4);
+            for (int w = 0; w < NW; ++w) {
+                const float mw = stat[w][16 * rt + row][0];
+                ll += stat[w][16 * rt + row][1] * (mw == mm || mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mw - mm) * cabs));      // (no maximum: 0 or NaN)
+            }
+            const float f = m[rt] == mm || m[rt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[rt] - mm) * cabs);
+            float *dst = &osum[wave][16 * rt + row][g * (D / 4)];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int t = 0; t < NB; ++t) po[r * NB + t] = (T)(l[rt] == 0.f ? 0.f : o[rt][t][r] * inv);
-                    if (a.lse && g == 0) a.lse[at[rt]] = l[rt] == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l[rt])) * 0.693147180559945f;
+                for (int t = 0; t < NB; t += 2) *reinterpret_cast<kv_f32x2 *>(dst + r * NB + t) = (kv_f32x2){o[rt][t][r] * f, o[rt][t + 1][r] * f};
+            if (wave == 0 && g == 0) {
+                whole[16 * rt + row][0] = mm == -INFINITY ? 0.f : mm * cabs;                  // (in units of log2)
+                whole[16 * rt + row][1] = ll;
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int e = tid; e < RT * 16 * (D / 4); e += 64 * NW) {
+            const int rr = e / (D / 4), d = e % (D / 4) * 4;
+            const int64_t to = place_of[rr];
+            if (to < 0) continue;
+            ta_f32x4 v = *reinterpret_cast<const ta_f32x4 *>(&osum[0][rr][d]);
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const ta_f32x4 *>(&osum[w][rr][d]);
+            const float mc = whole[rr][0], ll = whole[rr][1];
+            if (a.nsplit > 1) {
+                *reinterpret_cast<ta_f32x4 *>(a.part + ((int64_t)split * a.tokens * a.heads + to) * D + d) = v;
+                if (d == 0) {
+                    float *ml = a.part + (int64_t)a.nsplit * a.tokens * a.heads * D + ((int64_t)split * a.tokens * a.heads + to) * 2;
+                    ml[0] = ll == 0.f ? -INFINITY : mc;
+                    ml[1] = ll;
                 }
+            } else {
+                const float inv = ll == 0.f ? 0.f : 1.f / ll;
+                alignas(16) T x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = (T)(ll == 0.f ? 0.f : v[j] * inv);
+                T *po = static_cast<T *>(a.out) + to * D + d;
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<kv_u32x4 *>(po) = *reinterpret_cast<const kv_u32x4 *>(x);
+                else *reinterpret_cast<kv_u32x2 *>(po) = *reinterpret_cast<const kv_u32x2 *>(x);
+                if (a.lse && d == 0) a.lse[to] = ll == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(ll)) * 0.693147180559945f;
             }
         }
     }

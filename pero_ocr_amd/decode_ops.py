@@ -226,6 +226,10 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if want_lse else None
     if tokens:
         lib = _lib()
+        per16 = 16 // q.element_size()
+        if q.data_ptr() % 16 or qs[0] % per16 or qs[1] % per16:          # (the kernel loads 16 bytes at a time)
+            q = q.contiguous() if not q.is_contiguous() else q.clone()
+            qs = q.stride()
         args = _native.TreeAttentionArgs(
             q.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None, page_table.data_ptr(), lengths.data_ptr(), q_start.data_ptr(),
             mask.data_ptr() if mask is not None else None, None, 0, qs[0], qs[1], ps[0], mask.stride(0) if mask is not None else 0, tokens, int(max_queries),
