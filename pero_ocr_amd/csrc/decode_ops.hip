@@ -37,8 +37,8 @@ struct OnDevice {
     int was = -1;
     bool changed = false;
     int enter(int device_id) {
-        int n = 0;
-        if (hipGetDeviceCount(&n) != hipSuccess || n == 0) return refuse("no HIP device available: this library has no CPU fallback");
+        static const int n = [] { int c = 0; return hipGetDeviceCount(&c) == hipSuccess ? c : 0; }();
+        if (n == 0) return refuse("no HIP device available: this library has no CPU fallback");
         if (device_id < 0 || device_id >= n) return refuse("device_id %d out of range (%d devices)", device_id, n);
         if (hipGetDevice(&was) != hipSuccess) return refuse("hipGetDevice failed");
         if (was != device_id) {
