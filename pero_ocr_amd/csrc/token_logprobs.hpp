@@ -46,6 +46,12 @@ __device__ __forceinline__ uint32_t max16(uint32_t x) {
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
     return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
 }
+__device__ __forceinline__ float max16(float x) {
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false)));
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false)));
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, false)));
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, false)));
+}
 __device__ __forceinline__ float sum16(float x) {
     x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
     x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false));
@@ -75,25 +81,23 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
     const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     if (r >= a.rows) return;                                    // (whole groups of 16 lanes)
     const T *x = static_cast<const T *>(a.x) + r * a.stride;
-    uint32_t key[NV];
     float v[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = lane + 16 * i < a.C ? (float)x[lane + 16 * i] : 0.f;
-    uint32_t best = 0;
-#pragma unroll
     for (int i = 0; i < NV; ++i) {
-        key[i] = lane + 16 * i < a.C ? lp_key(v[i]) : 0u;       // (below the key of -inf)
-        best = max(best, key[i]);
+        v[i] = -INFINITY;
+        if (16 * i + 16 <= a.C || lane + 16 * i < a.C) v[i] = (float)x[lane + 16 * i];
     }
-    best = max16(best);
-    const float m = lp_value(best);
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, v[i]);
+    m = max16(m);
     const float base = m == -INFINITY ? 0.f : m;
     float z = 0.f, e = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const float d = v[i] - base, p = lane + 16 * i < a.C ? __builtin_amdgcn_exp2f(d * 1.44269504088896f) : 0.f;
+        const float d = v[i] - base, p = __builtin_amdgcn_exp2f(d * 1.44269504088896f);
         z += p;
-        e += p == 0.f ? 0.f : p * d;
+        e = fmaf(p, fmaxf(d, -200.f), e);                       // (p is 0 from -104 on)
     }
     z = sum16(z);
     e = sum16(e);
@@ -101,22 +105,49 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
     const float logz = __builtin_amdgcn_logf(z) * 0.693147180559945f;
     if (lane == 0) a.entropy[r] = none ? 0.f : logz - e / z;
     lp_given(a, r, lane, 16, base, logz, none);
-    for (int t = 0; t < a.top; ++t) {
+    float *top_lp = a.top_logprob + r * a.top;
+    int32_t *top_at = a.top_index + r * a.top;
+    // ---- the alternatives: rows of ordinary numbers by the numbers themselves, a taken one becomes -inf
+    bool plain = __ballot(!(z > 0.f && z <= 3.402823466e38f)) == 0;
+    float best = m;
+    for (int t = 0; plain && t < a.top; ++t) {
         if (t) {
-            best = 0;
+            best = v[0];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) best = max(best, key[i]);
+            for (int i = 1; i < NV; ++i) best = fmaxf(best, v[i]);
             best = max16(best);
+            if (__ballot(best == -INFINITY)) { plain = false; break; }          // fewer numbers than alternatives
         }
-        uint32_t low = 0;                                       // ~class: the largest is the lowest class
+        int slot = NV;
 #pragma unroll
-        for (int i = NV - 1; i >= 0; --i) low = key[i] == best ? ~(uint32_t)(lane + 16 * i) : low;
+        for (int i = NV - 1; i >= 0; --i) slot = v[i] == best ? i : slot;
+        const uint32_t mine = slot == NV ? 0u : ~(uint32_t)(lane + 16 * slot), low = max16(mine);          // ~class: the largest is the lowest class
+        slot = mine == low ? slot : NV;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = slot == i ? -INFINITY : v[i];
+        if (lane == 0) {
+            top_lp[t] = (best - base) - logz;
+            top_at[t] = (int32_t)~low;
+        }
+    }
+    if (plain) return;
+    // rows with NaN or infinities, or with fewer numbers than alternatives: by integer keys
+    uint32_t key[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) key[i] = lane + 16 * i < a.C ? lp_key((float)x[lane + 16 * i]) : 0u;          // (below the key of -inf)
+    for (int t = 0; t < a.top; ++t) {
+        uint32_t most = 0, low = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) most = max(most, key[i]);
+        most = max16(most);
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i) low = key[i] == most ? ~(uint32_t)(lane + 16 * i) : low;
         low = max16(low);
 #pragma unroll
         for (int i = 0; i < NV; ++i) key[i] = ~low == (uint32_t)(lane + 16 * i) ? 0u : key[i];
         if (lane == 0) {
-            a.top_logprob[r * a.top + t] = none ? -INFINITY : (lp_value(best) - base) - logz;
-            a.top_index[r * a.top + t] = (int32_t)~low;
+            top_lp[t] = none ? -INFINITY : (lp_value(most) - base) - logz;
+            top_at[t] = (int32_t)~low;
         }
     }
 }
