@@ -159,6 +159,28 @@ int check_attention(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
     return 0;
 }
 
+int check_scores(const pocr_token_logprobs_args *t) {
+    if (!t) return refuse("pocr_token_logprobs: NULL arguments");
+    if (!known_dtype(t->dtype)) return refuse("pocr_token_logprobs: dtype %d", t->dtype);
+    if (t->rows < 0 || t->rows > 0x7fffffff) return refuse("pocr_token_logprobs: rows %lld", (long long)t->rows);
+    if (t->classes < 1 || t->classes > 1 << 30) return refuse("pocr_token_logprobs: classes %d", t->classes);
+    if (t->given < 0) return refuse("pocr_token_logprobs: given %d", t->given);
+    if (t->top < 0 || t->top > LP_MAX_TOP || t->top > t->classes) return refuse("pocr_token_logprobs: top %d must be in 0..%d and at most the classes", t->top, LP_MAX_TOP);
+    return 0;
+}
+
+// Workgroups of a row: more than one where rows are too few to fill the chip and so long that one workgroup (36 GB/s) takes longer than
+// the second launch and the join (9 rows of 604 KB: whole 16.5 us, in slices 17.0 us).
+int score_slices(const pocr_token_logprobs_args *t) {
+    if ((int64_t)t->classes * elem_size(t->dtype) <= 786432 || t->rows >= 128) return 1;
+    return (int)std::min<int64_t>({(256 + t->rows - 1) / t->rows, t->classes / 8192, 64, LP_CAND / std::max(t->top, 1)});
+}
+
+int64_t score_workspace(const pocr_token_logprobs_args *t) {
+    const int64_t parts = t->rows * score_slices(t);
+    return parts == t->rows ? 0 : parts * (16 + 8 * (int64_t)t->top);
+}
+
 template <int DT> int score(void *stream, const LogprobArgs &a) {
     const char *w = "pocr_token_logprobs";
     const unsigned rows = (unsigned)a.rows;
@@ -166,7 +188,9 @@ template <int DT> int score(void *stream, const LogprobArgs &a) {
     if (a.C <= 512) return launch(w, token_logprobs_few_kernel<DT, 32>, dim3((rows + 15) / 16), dim3(256), stream, a);
     if (a.C <= 4096) return launch(w, token_logprobs_kernel<DT, 64>, dim3(rows), dim3(64), stream, a);
     if (a.C <= 32768) return launch(w, token_logprobs_kernel<DT, 256>, dim3(rows), dim3(256), stream, a);
-    return launch(w, token_logprobs_kernel<DT, 1024>, dim3(rows), dim3(1024), stream, a);
+    if (a.slices == 1) return launch(w, token_logprobs_kernel<DT, 1024>, dim3(rows), dim3(1024), stream, a);
+    if (launch(w, token_logprobs_kernel<DT, 256, true>, dim3(rows * a.slices), dim3(256), stream, a)) return 1;
+    return launch(w, token_logprobs_join_kernel<DT>, dim3(rows), dim3(256), stream, a);
 }
 
 }  // namespace
@@ -250,23 +274,25 @@ int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, con
     return go(std::integral_constant<int, DT_F16>());
 }
 
-int64_t pocr_token_logprobs_workspace(const pocr_token_logprobs_args *) { return 0; }
+int64_t pocr_token_logprobs_workspace(const pocr_token_logprobs_args *t) {
+    if (check_scores(t)) return -1;
+    return t->rows == 0 ? 0 : score_workspace(t);
+}
 
 int pocr_token_logprobs(int device_id, void *stream, const pocr_token_logprobs_args *t) {
-    if (!t) return refuse("pocr_token_logprobs: NULL arguments");
-    if (!known_dtype(t->dtype)) return refuse("pocr_token_logprobs: dtype %d", t->dtype);
-    if (t->rows < 0 || t->rows > 0x7fffffff) return refuse("pocr_token_logprobs: rows %lld", (long long)t->rows);
-    if (t->classes < 1 || t->classes > 1 << 30) return refuse("pocr_token_logprobs: classes %d", t->classes);
-    if (t->given < 0) return refuse("pocr_token_logprobs: given %d", t->given);
-    if (t->top < 0 || t->top > LP_MAX_TOP || t->top > t->classes) return refuse("pocr_token_logprobs: top %d must be in 0..%d and at most the classes", t->top, LP_MAX_TOP);
+    if (check_scores(t)) return 1;
     if (t->rows == 0) return 0;
     if (!t->logits || !t->entropy || (t->given > 0 && (!t->tokens || !t->logprob)) || (t->top > 0 && (!t->top_logprob || !t->top_index)))
         return refuse("pocr_token_logprobs: NULL pointer");
     if (!aligned(t->logits, elem_size(t->dtype)) || !aligned(t->tokens, t->tokens64 ? 8 : 4)) return refuse("pocr_token_logprobs: a pointer is not aligned to its element");
+    const int64_t need = score_workspace(t);
+    if (need > 0 && (!t->workspace || !aligned(t->workspace, 16) || t->workspace_bytes < need))
+        return refuse("pocr_token_logprobs: a workspace of %lld bytes, aligned to 16, is needed (pocr_token_logprobs_workspace)", (long long)need);
     OnDevice dev;
     if (dev.enter(device_id)) return 1;
+    const int slices = score_slices(t), slice = ((t->classes + slices - 1) / slices + 63) / 64 * 64;
     LogprobArgs a{t->logits, t->row_stride, t->tokens, t->logprob, t->entropy, t->top_logprob, t->top_index, t->rows, t->classes, t->given, t->top, t->tokens64,
-                  t->dtype};
+                  t->dtype, slices, slice, static_cast<float *>(t->workspace)};
     if (t->dtype == POCR_F32) return score<DT_F32>(stream, a);
     if (t->dtype == POCR_BF16) return score<DT_BF16>(stream, a);
     return score<DT_F16>(stream, a);

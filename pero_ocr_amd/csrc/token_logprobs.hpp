@@ -22,6 +22,8 @@ struct LogprobArgs {
     int32_t *top_index;               // [rows][top]
     int64_t rows;
     int32_t C, given, top, tokens64, dtype;
+    int32_t slices, slice;            // workgroups of a row, classes of each but the last
+    float *part;                      // slices > 1: [rows * slices][4] maximum, sum, weighted sum; then the alternatives [rows * slices][top] as 64-bit keys
 };
 
 constexpr int LP_MAX_TOP = 64;
@@ -158,6 +160,7 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
 // largest maximum T is kept and ranked.  Where many threads share T (equal logits, rows that are masked but for a few classes) the
 // numbers above T are kept and the lowest classes equal to T are found by reading the row from its start.  What does not fit
 // the list of candidates, and rows with NaN or +inf, take one pass per alternative.
+// Few long rows are cut into slices, a workgroup each (SPLIT), whose sums and alternatives the kernel below joins.
 constexpr int LP_CAND = 1024, LP_SLACK = 32;
 
 template <int DT, int V> __device__ __forceinline__ void lp_load(const void *p, float (&x)[V]) {
@@ -168,7 +171,7 @@ template <int DT, int V> __device__ __forceinline__ void lp_load(const void *p, 
     for (int i = 0; i < V; ++i) x[i] = (float)t[i];
 }
 
-template <int DT, int B>
+template <int DT, int B, bool SPLIT = false>
 __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     using T = typename ElemOf<DT>::type;
     constexpr int V = 16 / sizeof(T), W = B / 64, U = 4;
@@ -180,11 +183,12 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     __shared__ uint32_t limit[2];
     __shared__ int count[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = blockIdx.x;
-    const T *x = static_cast<const T *>(a.x) + r * a.stride;
+    const int64_t r = SPLIT ? blockIdx.x / (uint32_t)a.slices : blockIdx.x;
+    const int class0 = SPLIT ? (int)(blockIdx.x - (uint32_t)r * (uint32_t)a.slices) * a.slice : 0, C = SPLIT ? min(a.slice, a.C - class0) : a.C;
+    const T *x = static_cast<const T *>(a.x) + r * a.stride + class0;
     // head elements up to a multiple of 16 bytes, pieces, tail
     const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
-    const int head = min(off ? V - off : 0, a.C), pieces = (a.C - head) / V, tail = a.C - head - pieces * V;
+    const int head = min(off ? V - off : 0, C), pieces = (C - head) / V, tail = C - head - pieces * V;
     const T *body = x + head;
 
     float m = -INFINITY, ref = 0.f, z = 0.f, e = 0.f;
@@ -251,11 +255,19 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     const float base = m == -INFINITY ? 0.f : m;
     const bool none = z == 0.f, odd = !(z <= 3.402823466e38f);
     const float logz = __builtin_amdgcn_logf(z) * 0.693147180559945f;
-    if (tid == 0) a.entropy[r] = none ? 0.f : logz - e / z;
-    lp_given(a, r, tid, B, base, logz, none);
+    if constexpr (SPLIT) {
+        if (tid == 0) *reinterpret_cast<float4 *>(a.part + (int64_t)blockIdx.x * 4) = make_float4(m, z, e, 0.f);
+    } else {
+        if (tid == 0) a.entropy[r] = none ? 0.f : logz - e / z;
+        lp_given(a, r, tid, B, base, logz, none);
+    }
     const int k = a.top;
     if (k == 0) return;
     auto put = [&](int at, unsigned long long c) {
+        if constexpr (SPLIT) {
+            reinterpret_cast<unsigned long long *>(a.part + (int64_t)a.rows * a.slices * 4)[(int64_t)blockIdx.x * k + at] = c - (uint32_t)class0;      // (low word: ~class)
+            return;
+        }
         a.top_logprob[r * k + at] = none ? -INFINITY : (lp_value((uint32_t)(c >> 32)) - base) - logz;
         a.top_index[r * k + at] = (int32_t)~(uint32_t)c;
     };
@@ -313,9 +325,9 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
         bool fits = n <= LP_CAND;
         if (ties && n < k) {                                    // the lowest classes equal to T0 make up the rest
             __syncthreads();
-            for (int c0 = 0; c0 < a.C && n < k; c0 += B) {
+            for (int c0 = 0; c0 < C && n < k; c0 += B) {
                 const int c = c0 + tid;
-                if (c < a.C && lp_key((float)x[c]) == T0) cand[atomicAdd(&count[1], 1)] = (unsigned long long)T0 << 32 | (uint32_t)~c;
+                if (c < C && lp_key((float)x[c]) == T0) cand[atomicAdd(&count[1], 1)] = (unsigned long long)T0 << 32 | (uint32_t)~c;
                 __syncthreads();
                 n = count[1];                                   // (at most k - 1 + B)
                 __syncthreads();
@@ -335,7 +347,7 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     unsigned long long last = ~0ull;                            // (key, ~class) of the previous alternative
     for (int t = 0; t < k; ++t) {
         unsigned long long b = 0;
-        for (int c = tid; c < a.C; c += B) {
+        for (int c = tid; c < C; c += B) {
             const unsigned long long q = (unsigned long long)lp_key((float)x[c]) << 32 | (uint32_t)~c;
             if ((t == 0 || q < last) && q > b) b = q;
         }
@@ -346,6 +358,48 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
         for (int w = 0; w < W; ++w) b = cand[w] > b ? cand[w] : b;
         last = b;
         if (tid == 0) put(t, b);
+    }
+}
+
+// The slices of a row meet: a workgroup per row; a lane per slice for the sums, the alternatives ranked among all slices'.
+template <int DT>
+__global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogprobArgs a) {
+    __shared__ unsigned long long cand[LP_CAND];
+    __shared__ float whole[2];
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    const int n = a.slices * a.top;                             // <= LP_CAND
+    const unsigned long long *found = reinterpret_cast<const unsigned long long *>(a.part + a.rows * a.slices * 4) + r * n;
+    for (int i = tid; i < n; i += 256) cand[i] = found[i];
+    if (tid < 64) {                                             // (slices <= 64)
+        float4 s = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        if (tid < a.slices) s = *reinterpret_cast<const float4 *>(a.part + (r * a.slices + tid) * 4);
+        float m = s.x, z = s.y, e = s.z;
+        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const float d = s.x == -INFINITY ? 0.f : s.x - m, f = __builtin_amdgcn_exp2f(d * 1.44269504088896f);
+        e = f == 0.f && z == z ? 0.f : f * fmaf(d, z, e);
+        z *= f;
+        for (int o = 32; o >= 1; o >>= 1) { z += __shfl_xor(z, o, 64); e += __shfl_xor(e, o, 64); }
+        if (tid == 0) {
+            const bool none = z == 0.f;
+            const float logz = __builtin_amdgcn_logf(z) * 0.693147180559945f;
+            a.entropy[r] = none ? 0.f : logz - e / z;
+            whole[0] = m;
+            whole[1] = none ? -INFINITY : logz;                 // (an ordinary row's is not below 0)
+        }
+    }
+    __syncthreads();
+    const float m = whole[0], base = m == -INFINITY ? 0.f : m, logz = whole[1];
+    const bool none = logz == -INFINITY;
+    lp_given(a, r, tid, 256, base, logz, none);
+    for (int i = tid; i < n; i += 256) {
+        const unsigned long long c = cand[i];
+        int rank = 0;
+        for (int q = 0; q < n; ++q) rank += cand[q] > c;
+        if (rank < a.top) {
+            a.top_logprob[r * a.top + rank] = none ? -INFINITY : (lp_value((uint32_t)(c >> 32)) - base) - logz;
+            a.top_index[r * a.top + rank] = (int32_t)~(uint32_t)c;
+        }
     }
 }
 

@@ -64,6 +64,19 @@ def test_c_entries_refuse_bad_arguments():
         base.update(kw)
         assert lib.pocr_token_logprobs(0, None, _native.TokenLogprobsArgs(**base)) == 1 and word in _err(), kw
     assert lib.pocr_token_logprobs(0, None, None) == 1 and "NULL" in _err()
+    # scratch memory that is needed and not given, too small or not aligned
+    args = _native.TokenLogprobsArgs(logits=p, tokens=p, logprob=p, entropy=p, top_logprob=p, top_index=p, row_stride=1 << 19, rows=2, classes=1 << 19, given=1, top=2)
+    need = lib.pocr_token_logprobs_workspace(args)
+    assert need > 0
+    for w, n in ((None, need), (p, need - 1), (p + 8, need)):
+        args.workspace, args.workspace_bytes = w, n
+        assert lib.pocr_token_logprobs(0, None, args) == 1 and "workspace" in _err()
+    args = _native.TreeAttentionArgs(q=p, out=p, page_table=p, lengths=p, q_start=p, tokens=1, seqs=1, heads=2, max_pages=4096, q_head_stride=64, q_token_stride=128)
+    need = lib.pocr_tree_attention_workspace(pages, args)
+    assert need > 0
+    for w, n in ((None, need), (p, need - 1), (p + 8, need)):
+        args.workspace, args.workspace_bytes = w, n
+        assert lib.pocr_tree_attention(0, None, pages, args) == 1 and "workspace" in _err()
 
 
 def test_python_refusals_on_cpu_tensors():
@@ -559,6 +572,35 @@ def test_gpu_logprobs_hard_orders(rows, order):
     got = ops.token_logprobs(x, tokens, top=50)
     assert all((t == t[:1]).all() for t in got[1:])
     _check_scores(x[:1], tokens[:1], 50, [t[:1] for t in got])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows, classes, top", [(1, 32769, 64), (1, 600000, 3), (2, 140003, 16), (9, 400009, 64), (127, 200001, 7), (128, 200001, 7), (9, 500001, 0)])
+def test_gpu_logprobs_few_long_rows(rows, classes, top, kind):
+    """rows that are cut into slices: special rows among ordinary ones, the alternatives in one slice or in several, given tokens in any"""
+    g = _gen(rows)
+    x = (torch.randn(rows, classes, device="cuda", generator=g) * 2).to(TYPES[kind])
+    for r in range(min(rows, 9)):
+        if r == 1:
+            x[r, 50:] = -math.inf
+        elif r == 2:
+            x[r] = -math.inf
+        elif r == 3:
+            x[r, classes - 3] = math.nan
+        elif r == 4:
+            x[r, 20000:20100] = 11.0
+        elif r == 5:
+            x[r] = 1.5
+        elif r == 6:
+            x[r, 8] = math.inf
+        elif r == 7:
+            x[r, :30000] = math.nan
+    tokens = torch.randint(0, classes, (rows, 2), device="cuda", generator=g)
+    tokens[0, 1] = classes - 1
+    at = list(range(min(rows, 9)))
+    got = ops.token_logprobs(x, tokens, top=top)
+    _check_scores(x[at], tokens[at], top, [t[at] for t in got])
 
 
 @pytest.mark.gpu
