@@ -392,11 +392,15 @@ typedef struct pocr_kv_pages {
     uint8_t *k_exp, *v_exp;
     int32_t num_pages, kv_heads, page_size, head_dim, format;
 } pocr_kv_pages;
-/* k, v [tokens][kv_heads][head_dim] with element strides per token and head (the last axis is contiguous) -> the rows of slots[tokens]
- * (int64 when slots64, else int32).  A slot outside the cache (-1: padding) is skipped.  Slots of one call are distinct: a slot
- * named twice holds a mixture of the rows given for it. */
-int pocr_kv_write(int device_id, void *stream, const pocr_kv_pages *pages, const void *k, const void *v, int32_t dtype, int64_t k_token_stride,
-                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void *slots, int32_t slots64, int64_t tokens);
+/* Keys and values to be written: k, v [tokens][kv_heads][head_dim] of `dtype` with element strides per token and head (the last axis is
+ * contiguous) -> the rows of slots[tokens] (int64 when slots64, else int32).  A slot outside the cache (-1: padding) is skipped.  Slots of
+ * one call are distinct: a slot named twice holds a mixture of the rows given for it. */
+typedef struct pocr_kv_rows {
+    const void *k, *v, *slots;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride, tokens;
+    int32_t dtype, slots64;
+} pocr_kv_rows;
+int pocr_kv_write(int device_id, void *stream, const pocr_kv_pages *pages, const pocr_kv_rows *rows);
 /* The rows of slots[tokens] -> k, v [tokens][kv_heads][head_dim] (contiguous, 16-byte aligned) as `dtype`, rounded to nearest even; a
  * slot outside the cache reads as zeros. */
 int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const void *slots, int32_t slots64, int64_t tokens, void *k, void *v,

@@ -47,6 +47,12 @@ class KvPages(C.Structure):
                 ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("format", C.c_int32)]
 
 
+class KvRows(C.Structure):
+    """pocr_kv_rows (include/pocr.h): keys and values to be written, and where."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("slots", C.c_void_p), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64), ("tokens", C.c_int64), ("dtype", C.c_int32), ("slots64", C.c_int32)]
+
+
 class TreeAttentionArgs(C.Structure):
     """pocr_tree_attention_args (include/pocr.h)."""
     _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
@@ -111,8 +117,7 @@ SYMBOLS = {
     "pocr_cropper_read_curves": (C.c_int, [C.c_void_p, C.POINTER(C.c_double), C.c_int64]),
     "pocr_cropper_last_ms": (C.c_float, [C.c_void_p]),
     "pocr_num_slots": (C.c_int, []),
-    "pocr_kv_write": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(KvPages), C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64,
-                                C.c_int64, C.c_void_p, C.c_int32, C.c_int64]),
+    "pocr_kv_write": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(KvPages), C.POINTER(KvRows)]),
     "pocr_kv_read": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(KvPages), C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32]),
     "pocr_tree_attention_workspace": (C.c_int64, [C.POINTER(KvPages), C.POINTER(TreeAttentionArgs)]),
     "pocr_tree_attention": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(KvPages), C.POINTER(TreeAttentionArgs)]),

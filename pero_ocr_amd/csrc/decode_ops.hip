@@ -197,21 +197,22 @@ template <int DT> int score(void *stream, const LogprobArgs &a) {
 
 extern "C" {
 
-int pocr_kv_write(int device_id, void *stream, const pocr_kv_pages *c, const void *k, const void *v, int32_t dtype, int64_t k_token_stride,
-                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void *slots, int32_t slots64, int64_t tokens) {
-    if (check_pages(c) || check_rows(c, tokens, "pocr_kv_write")) return 1;
-    if (!known_dtype(dtype)) return refuse("pocr_kv_write: dtype %d", dtype);
-    if (tokens == 0) return 0;
-    if (!k || !v || !slots) return refuse("pocr_kv_write: NULL pointer");
-    const int es = elem_size(dtype);
-    if (!aligned(k, es) || !aligned(v, es) || !aligned(slots, slots64 ? 8 : 4)) return refuse("pocr_kv_write: a pointer is not aligned to its element");
+int pocr_kv_write(int device_id, void *stream, const pocr_kv_pages *c, const pocr_kv_rows *t) {
+    if (check_pages(c)) return 1;
+    if (!t) return refuse("pocr_kv_write: NULL arguments");
+    if (check_rows(c, t->tokens, "pocr_kv_write")) return 1;
+    if (!known_dtype(t->dtype)) return refuse("pocr_kv_write: dtype %d", t->dtype);
+    if (t->tokens == 0) return 0;
+    if (!t->k || !t->v || !t->slots) return refuse("pocr_kv_write: NULL pointer");
+    const int es = elem_size(t->dtype), dtype = t->dtype;
+    if (!aligned(t->k, es) || !aligned(t->v, es) || !aligned(t->slots, t->slots64 ? 8 : 4)) return refuse("pocr_kv_write: a pointer is not aligned to its element");
     OnDevice dev;
     if (dev.enter(device_id)) return 1;
-    KvWriteArgs a{c->k, c->v, c->k_exp, c->v_exp, k, v, slots, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
-                  c->num_pages, c->kv_heads, page_shift(c), (uint32_t)(tokens * 2 * c->kv_heads), slots64};
+    KvWriteArgs a{c->k, c->v, c->k_exp, c->v_exp, t->k, t->v, t->slots, t->k_token_stride, t->k_head_stride, t->v_token_stride, t->v_head_stride,
+                  c->num_pages, c->kv_heads, page_shift(c), (uint32_t)(t->tokens * 2 * c->kv_heads), t->slots64};
     // 16-byte loads where every row starts at a multiple of 16 bytes, single elements otherwise
-    const bool vec = aligned(k, 16) && aligned(v, 16) && (k_token_stride * es) % 16 == 0 && (k_head_stride * es) % 16 == 0 &&
-                     (v_token_stride * es) % 16 == 0 && (v_head_stride * es) % 16 == 0;
+    const bool vec = aligned(t->k, 16) && aligned(t->v, 16) && (t->k_token_stride * es) % 16 == 0 && (t->k_head_stride * es) % 16 == 0 &&
+                     (t->v_token_stride * es) % 16 == 0 && (t->v_head_stride * es) % 16 == 0;
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         if (c->format == POCR_KV_FP8) return vec ? write_by_dim<DT, KV_FP8, true>(row_grid, c->head_dim, stream, a) : write_by_dim<DT, KV_FP8, false>(row_grid, c->head_dim, stream, a);

@@ -30,6 +30,8 @@ from . import _native
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FORMATS = {torch.bfloat16: 0, torch.float8_e4m3fn: 1}
+_BF16, _FP8, _BYTE, _INT, _LONG = torch.bfloat16, torch.float8_e4m3fn, torch.uint8, torch.int32, torch.int64
+_IDS = (_LONG, _INT)
 MAX_TOP = 64
 
 _checked_lib = None
@@ -59,9 +61,8 @@ _Tensor = torch.Tensor
 
 
 def _need(t, name: str, device: Optional[torch.device], dtypes, dims: int):
-    """The checks that every tensor argument has to pass, one short expression where they do."""
-    if type(t) is _Tensor and t.dtype in dtypes and t.dim() == dims and not t.requires_grad and (t.device == device if device is not None else t.is_cuda):
-        return
+    """The checks that every tensor argument has to pass, with the reason where one does not.  (Called where a short expression of the
+    caller's says that something is wrong: a call of these operators takes as long on the host as on the GPU.)"""
     if not isinstance(t, _Tensor):
         raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
@@ -77,48 +78,52 @@ def _need(t, name: str, device: Optional[torch.device], dtypes, dims: int):
         raise RuntimeError(f"{name} requires a gradient: the decoding operators are for inference (use torch.no_grad())")
 
 
-_IDS = (torch.int64, torch.int32)
-_I32 = (torch.int32,)
-_I64 = (torch.int64,)
-_U8 = (torch.uint8,)
 
 
 class KVPages:
     """One layer's cache: k, v [pages, kv_heads, page_size, head_dim], bfloat16 or float8_e4m3fn; in 8 bits k_exp, v_exp uint8
     [pages, kv_heads, page_size] hold the power of two of every row: it stands for code * 2 ** (exp - 127).  Slot s is row
     s % page_size of page s // page_size.  The tensors stay the caller's (contiguous, same device); kv_pages() makes them."""
-    __slots__ = ("k", "v", "k_exp", "v_exp", "device", "index", "native")
+    __slots__ = ("k", "v", "k_exp", "v_exp", "index", "native")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None):
-        _need(k, "k", None, _FORMATS, 4)
-        device, dtype, shape = k.device, k.dtype, k.shape
-        _need(v, "v", device, (dtype,), 4)
-        if v.shape != shape:
-            raise ValueError(f"k and v differ in shape: {tuple(shape)}, {tuple(v.shape)}")
-        whole = k.is_contiguous() and v.is_contiguous()
-        if dtype is torch.float8_e4m3fn:
-            _need(k_exp, "k_exp", device, _U8, 3)
-            _need(v_exp, "v_exp", device, _U8, 3)
-            rows = shape[:3]
-            if k_exp.shape != rows or v_exp.shape != rows:
-                raise ValueError(f"k_exp, v_exp: expected shape {tuple(rows)}, got {tuple(k_exp.shape)}, {tuple(v_exp.shape)}")
-            whole = whole and k_exp.is_contiguous() and v_exp.is_contiguous()
-            exps = k_exp.data_ptr(), v_exp.data_ptr()
-        elif k_exp is not None or v_exp is not None:
-            raise ValueError("a bfloat16 cache has no exponents")
-        else:
-            exps = None, None
-        if not whole:
-            raise ValueError("the cache's tensors must be contiguous")
-        n, h, p, d = shape
+        fp8 = k_exp is not None
+        if not (type(k) is _Tensor and type(v) is _Tensor and k.is_cuda and k.dtype is (_FP8 if fp8 else _BF16) and v.dtype is k.dtype
+                and k.dim() == 4 and k.shape == v.shape and v.get_device() == k.get_device() and k.is_contiguous() and v.is_contiguous()
+                and not (k.requires_grad or v.requires_grad)
+                and (type(k_exp) is _Tensor and type(v_exp) is _Tensor and k_exp.dtype is _BYTE and v_exp.dtype is _BYTE
+                     and k_exp.shape == v_exp.shape == k.shape[:3] and k_exp.get_device() == k.get_device() == v_exp.get_device()
+                     and k_exp.is_contiguous() and v_exp.is_contiguous() if fp8 else v_exp is None)):
+            self._refuse(k, v, k_exp, v_exp)
+        n, h, p, d = k.shape
         if d not in (32, 64, 128, 256):
             raise ValueError(f"head_dim {d}: 32, 64, 128 or 256")
         if p < 16 or p & (p - 1):
             raise ValueError(f"page_size {p}: a power of two from 16 on")
         if n < 1 or h < 1:
-            raise ValueError(f"an empty cache: {tuple(shape)}")
-        self.k, self.v, self.k_exp, self.v_exp, self.device, self.index = k, v, k_exp, v_exp, device, device.index
-        self.native = _native.KvPages(k.data_ptr(), v.data_ptr(), exps[0], exps[1], n, h, p, d, _FORMATS[dtype])
+            raise ValueError(f"an empty cache: {tuple(k.shape)}")
+        self.k, self.v, self.k_exp, self.v_exp, self.index = k, v, k_exp, v_exp, k.get_device()
+        self.native = _native.KvPages(k.data_ptr(), v.data_ptr(), k_exp.data_ptr() if fp8 else None, v_exp.data_ptr() if fp8 else None, n, h, p, d, fp8)
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
+    @staticmethod
+    def _refuse(k, v, k_exp, v_exp):
+        _need(k, "k", None, _FORMATS, 4)
+        _need(v, "v", k.device, (k.dtype,), 4)
+        if v.shape != k.shape:
+            raise ValueError(f"k and v differ in shape: {tuple(k.shape)}, {tuple(v.shape)}")
+        if k.dtype is _FP8:
+            _need(k_exp, "k_exp", k.device, (_BYTE,), 3)
+            _need(v_exp, "v_exp", k.device, (_BYTE,), 3)
+            if k_exp.shape != k.shape[:3] or v_exp.shape != k.shape[:3]:
+                raise ValueError(f"k_exp, v_exp: expected shape {tuple(k.shape[:3])}, got {tuple(k_exp.shape)}, {tuple(v_exp.shape)}")
+        elif k_exp is not None or v_exp is not None:
+            raise ValueError("a bfloat16 cache has no exponents")
+        if not all(t.is_contiguous() for t in (k, v, k_exp, v_exp) if t is not None):
+            raise ValueError("the cache's tensors must be contiguous")
 
 
 def kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: str = "fp8", device="cuda") -> KVPages:
@@ -133,10 +138,11 @@ def kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype
 
 
 def _check_slots(slots, pages: KVPages) -> int:
-    _need(slots, "slots", pages.device, _IDS, 1)
+    if not (type(slots) is _Tensor and slots.dtype in _IDS and slots.dim() == 1 and slots.get_device() == pages.index):
+        _need(slots, "slots", pages.device, _IDS, 1)
     if not slots.is_contiguous():
         raise ValueError("slots must be contiguous")
-    return slots.shape[0]
+    return slots.numel()
 
 
 def kv_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -144,18 +150,20 @@ def kv_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
     projection) into the cache's format and stores them at slots [tokens].  A slot outside the cache (-1 for padding) is skipped; the
     slots of one call are distinct."""
     tokens = _check_slots(slots, pages)
-    _need(k, "k", pages.device, _DTYPES, 3)
-    _need(v, "v", pages.device, (k.dtype,), 3)
-    n = pages.native
-    shape = (tokens, n.kv_heads, n.head_dim)
-    if k.shape != shape or v.shape != shape:
-        raise ValueError(f"k, v: expected shape {shape}, got {tuple(k.shape)}, {tuple(v.shape)}")
+    n, index = pages.native, pages.index
+    if not (type(k) is _Tensor and type(v) is _Tensor and k.dtype in _DTYPES and v.dtype is k.dtype and k.dim() == 3 == v.dim()
+            and k.get_device() == index == v.get_device() and not (k.requires_grad or v.requires_grad)):
+        _need(k, "k", pages.device, _DTYPES, 3)
+        _need(v, "v", pages.device, (k.dtype,), 3)
+    shape = k.shape
+    if shape != v.shape or shape[0] != tokens or shape[1] != n.kv_heads or shape[2] != n.head_dim:
+        raise ValueError(f"k, v: expected shape {(tokens, n.kv_heads, n.head_dim)}, got {tuple(shape)}, {tuple(v.shape)}")
     kt, kh, k1 = k.stride()
     vt, vh, v1 = v.stride()
     if k1 != 1 or v1 != 1:
         raise ValueError("the last axis of k and v must be contiguous")
-    if _lib().pocr_kv_write(pages.index, _stream(pages.index), n, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], kt, kh, vt, vh, slots.data_ptr(),
-                            slots.dtype is torch.int64, tokens):
+    rows = _native.KvRows(k.data_ptr(), v.data_ptr(), slots.data_ptr(), kt, kh, vt, vh, tokens, _DTYPES[k.dtype], slots.dtype is _LONG)
+    if _lib().pocr_kv_write(index, _stream(index), n, rows):
         _fail("pocr_kv_write")
 
 
@@ -164,10 +172,10 @@ def kv_read(pages: KVPages, slots: torch.Tensor, dtype: torch.dtype = torch.floa
     tokens = _check_slots(slots, pages)
     if dtype not in _DTYPES:
         raise TypeError(f"dtype {dtype}: float32, bfloat16 or float16")
-    n = pages.native
-    k = torch.empty((tokens, n.kv_heads, n.head_dim), dtype=dtype, device=pages.device)
+    n, index = pages.native, pages.index
+    k = pages.k.new_empty((tokens, n.kv_heads, n.head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    if _lib().pocr_kv_read(pages.index, _stream(pages.index), n, slots.data_ptr(), slots.dtype is torch.int64, tokens, k.data_ptr(), v.data_ptr(), _DTYPES[dtype]):
+    if _lib().pocr_kv_read(index, _stream(index), n, slots.data_ptr(), slots.dtype is _LONG, tokens, k.data_ptr(), v.data_ptr(), _DTYPES[dtype]):
         _fail("pocr_kv_read")
     return k, v
 
@@ -204,32 +212,37 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
 
     -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros
     (lse -inf) in a tensor made here and are left alone in an `out` of the caller's (contiguous)."""
-    n, device = pages.native, pages.device
-    _need(q, "q", device, _DTYPES, 3)
-    _need(page_table, "page_table", device, _I32, 2)
-    _need(lengths, "lengths", device, _I32, 1)
-    _need(q_start, "q_start", device, _I32, 1)
+    n, index = pages.native, pages.index
+    if not (type(q) is _Tensor and type(page_table) is _Tensor and type(lengths) is _Tensor and type(q_start) is _Tensor and q.dtype in _DTYPES
+            and page_table.dtype is _INT and lengths.dtype is _INT and q_start.dtype is _INT and q.dim() == 3 and page_table.dim() == 2
+            and lengths.dim() == 1 and q_start.dim() == 1 and not q.requires_grad
+            and q.get_device() == page_table.get_device() == lengths.get_device() == q_start.get_device() == index):
+        device = pages.device
+        _need(q, "q", device, _DTYPES, 3)
+        _need(page_table, "page_table", device, (_INT,), 2)
+        _need(lengths, "lengths", device, (_INT,), 1)
+        _need(q_start, "q_start", device, (_INT,), 1)
     tokens, heads, dim = q.shape
     seqs, width = page_table.shape
     if dim != n.head_dim or heads < 1 or heads % n.kv_heads:
         raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {n.kv_heads} key heads of {n.head_dim}")
-    if lengths.shape[0] != seqs or q_start.shape[0] != seqs + 1:
+    if lengths.numel() != seqs or q_start.numel() != seqs + 1:
         raise ValueError(f"page_table {tuple(page_table.shape)} and q_start {tuple(q_start.shape)} do not fit {seqs} sequences")
     qs, ps = q.stride(), page_table.stride()
     if qs[2] != 1 or (width > 1 and ps[1] != 1) or not lengths.is_contiguous() or not q_start.is_contiguous():
         raise ValueError("the last axis of q, page_table, lengths and q_start must be contiguous")
     if mask is not None:
-        _need(mask, "mask", device, _I64, 2)
+        _need(mask, "mask", pages.device, (_LONG,), 2)
         if mask.shape[0] != tokens or (tokens and mask.shape[1] < 1) or (mask.shape[1] > 1 and mask.stride(1) != 1):
             raise ValueError(f"mask: expected [{tokens}, at least one word] with a contiguous last axis, got {tuple(mask.shape)}")
     fresh = out is None
     if fresh:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
+        out = q.new_empty((tokens, heads, dim))
     else:
-        _need(out, "out", device, (q.dtype,), 3)
+        _need(out, "out", pages.device, (q.dtype,), 3)
         if out.shape != q.shape or not out.is_contiguous():
             raise ValueError(f"out: expected a contiguous tensor of shape {tuple(q.shape)}")
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if want_lse else None
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if want_lse else None
     if tokens:
         lib = _lib()
         at = q.data_ptr()
@@ -245,9 +258,9 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
         if need:
             if need < 0:
                 _fail("pocr_tree_attention")
-            scratch = torch.empty((need,), dtype=torch.uint8, device=device)
+            scratch = q.new_empty((need,), dtype=_BYTE)
             args.workspace, args.workspace_bytes = scratch.data_ptr(), need
-        if lib.pocr_tree_attention(pages.index, _stream(pages.index), n, args):
+        if lib.pocr_tree_attention(index, _stream(index), n, args):
             _fail("pocr_tree_attention")
     return (out, lse) if want_lse else out
 
@@ -259,11 +272,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     padding; NaN for one beyond the classes); entropy float32 [rows] of softmax(row); top_logprob float32 and top_index int32 [rows, top], the
     `top` <= 64 likeliest classes, equally likely ones in the order of their index.  A logit of -inf has probability 0; a row of nothing else
     has log probabilities -inf and entropy 0; a row with NaN or +inf has NaN."""
-    _need(logits, "logits", None, _DTYPES, 2)
-    device = logits.device
-    if not isinstance(tokens, _Tensor) or tokens.dim() not in (1, 2):
-        raise ValueError("tokens: expected a tensor [rows] or [rows, given]")
-    _need(tokens, "tokens", device, _IDS, tokens.dim())
+    if not (type(logits) is _Tensor and type(tokens) is _Tensor and logits.is_cuda and logits.dtype in _DTYPES and logits.dim() == 2 and tokens.dtype in _IDS
+            and 1 <= tokens.dim() <= 2 and tokens.get_device() == logits.get_device() and not logits.requires_grad):
+        _need(logits, "logits", None, _DTYPES, 2)
+        _need(tokens, "tokens", logits.device, _IDS, 2 if isinstance(tokens, _Tensor) and tokens.dim() == 2 else 1)
     rows, classes = logits.shape
     shape = tokens.shape
     if shape[0] != rows or not tokens.is_contiguous():
@@ -273,21 +285,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     stride, last = logits.stride()
     if classes > 1 and last != 1:
         raise ValueError("the last axis of logits must be contiguous")
-    logprob = torch.empty(shape, dtype=torch.float32, device=device)
+    logprob = logits.new_empty(shape, dtype=torch.float32)
     entropy = logprob.new_empty((rows,))
     top_logprob = logprob.new_empty((rows, top))
-    top_index = torch.empty((rows, top), dtype=torch.int32, device=device)
+    top_index = logprob.new_empty((rows, top), dtype=_INT)
     if rows:
         lib = _lib()
         args = _native.TokenLogprobsArgs(
             logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), None, 0, stride, rows,
-            _DTYPES[logits.dtype], classes, shape[1] if len(shape) == 2 else 1, top, tokens.dtype is torch.int64)
+            _DTYPES[logits.dtype], classes, shape[1] if len(shape) == 2 else 1, top, tokens.dtype is _LONG)
         need = lib.pocr_token_logprobs_workspace(args)
         if need:
             if need < 0:
                 _fail("pocr_token_logprobs")
-            scratch = torch.empty((need,), dtype=torch.uint8, device=device)
+            scratch = logits.new_empty((need,), dtype=_BYTE)
             args.workspace, args.workspace_bytes = scratch.data_ptr(), need
-        if lib.pocr_token_logprobs(device.index, _stream(device.index), args):
+        index = logits.get_device()
+        if lib.pocr_token_logprobs(index, _stream(index), args):
             _fail("pocr_token_logprobs")
     return logprob, entropy, top_logprob, top_index

@@ -34,7 +34,7 @@ def _err():
 def test_c_entries_refuse_a_bad_cache(kw, word):
     lib, pages = _native.load(), _fake_pages(**kw)
     p = 1 << 20
-    assert lib.pocr_kv_write(0, None, pages, p, p, 0, 128, 64, 128, 64, p, 1, 3) == 1 and word in _err()
+    assert lib.pocr_kv_write(0, None, pages, _native.KvRows(p, p, p, 128, 64, 128, 64, 3, 0, 1)) == 1 and word in _err()
     assert lib.pocr_kv_read(0, None, pages, p, 1, 3, p, p, 0) == 1 and word in _err()
     args = _native.TreeAttentionArgs(q=p, out=p, page_table=p, lengths=p, q_start=p, tokens=1, seqs=1, heads=2, max_pages=1)
     assert lib.pocr_tree_attention(0, None, pages, args) == 1 and word in _err()
@@ -43,12 +43,13 @@ def test_c_entries_refuse_a_bad_cache(kw, word):
 
 def test_c_entries_refuse_bad_arguments():
     lib, pages, p = _native.load(), _fake_pages(), 1 << 20
-    assert lib.pocr_kv_write(0, None, pages, p, p, 7, 128, 64, 128, 64, p, 1, 3) == 1 and "dtype" in _err()
-    assert lib.pocr_kv_write(0, None, pages, p + 1, p, 1, 128, 64, 128, 64, p, 1, 3) == 1 and "aligned" in _err()
-    assert lib.pocr_kv_write(0, None, pages, p, p, 0, 128, 64, 128, 64, None, 1, 3) == 1 and "NULL" in _err()
-    assert lib.pocr_kv_write(0, None, pages, p, p, 0, 128, 64, 128, 64, p, 1, -1) == 1 and "tokens" in _err()
-    assert lib.pocr_kv_write(0, None, pages, p, p, 0, 128, 64, 128, 64, p, 1, 1 << 40) == 1 and "2^31" in _err()
-    assert lib.pocr_kv_write(0, None, pages, None, None, 0, 128, 64, 128, 64, None, 1, 0) == 0          # nothing to do
+    for kw, word in ((dict(dtype=7), "dtype"), (dict(k=p + 1, dtype=1), "aligned"), (dict(slots=p + 4), "aligned"), (dict(slots=None), "NULL"), (dict(v=None), "NULL"),
+                     (dict(tokens=-1), "tokens"), (dict(tokens=1 << 40), "2^31")):
+        base = dict(k=p, v=p, slots=p, k_token_stride=128, k_head_stride=64, v_token_stride=128, v_head_stride=64, tokens=3, dtype=0, slots64=1)
+        base.update(kw)
+        assert lib.pocr_kv_write(0, None, pages, _native.KvRows(**base)) == 1 and word in _err(), kw
+    assert lib.pocr_kv_write(0, None, pages, None) == 1 and "NULL" in _err()
+    assert lib.pocr_kv_write(0, None, pages, _native.KvRows(tokens=0)) == 0                              # nothing to do
     assert lib.pocr_kv_read(0, None, pages, p, 1, 3, p + 4, p, 0) == 1 and "16 bytes" in _err()
     assert lib.pocr_kv_read(0, None, pages, p, 1, 3, p, p, 3) == 1 and "dtype" in _err()
     for kw, word in ((dict(q=None), "NULL"), (dict(lengths=None), "NULL"), (dict(page_table=None), "NULL"), (dict(heads=3), "heads"), (dict(heads=0), "heads"),
