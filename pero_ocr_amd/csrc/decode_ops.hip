@@ -101,7 +101,8 @@ template <int DT, int FMT> int read_by_dim(dim3 (*grid)(uint32_t, int), int D, v
     }
 }
 
-dim3 row_grid(uint32_t rows, int D) { const uint32_t per = 256 / (D / 8); return dim3((rows + per - 1) / per); }
+// workgroups for `rows` rows of D elements, E of them a lane
+template <int E> dim3 row_grid(uint32_t rows, int D) { const uint32_t per = 256 / (D / E); return dim3((rows + per - 1) / per); }
 
 // 32 rows a wave where their queries and sums leave room for two waves in a SIMD's registers
 constexpr bool two_tiles(int dtype, int D) { return D <= 64 || (D == 128 && dtype != POCR_F32); }
@@ -215,8 +216,8 @@ int pocr_kv_write(int device_id, void *stream, const pocr_kv_pages *c, const poc
                      (t->v_token_stride * es) % 16 == 0 && (t->v_head_stride * es) % 16 == 0;
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (c->format == POCR_KV_FP8) return vec ? write_by_dim<DT, KV_FP8, true>(row_grid, c->head_dim, stream, a) : write_by_dim<DT, KV_FP8, false>(row_grid, c->head_dim, stream, a);
-        return vec ? write_by_dim<DT, KV_BF16, true>(row_grid, c->head_dim, stream, a) : write_by_dim<DT, KV_BF16, false>(row_grid, c->head_dim, stream, a);
+        if (c->format == POCR_KV_FP8) return vec ? write_by_dim<DT, KV_FP8, true>(row_grid<KV_WRITE_ELEMS>, c->head_dim, stream, a) : write_by_dim<DT, KV_FP8, false>(row_grid<KV_WRITE_ELEMS>, c->head_dim, stream, a);
+        return vec ? write_by_dim<DT, KV_BF16, true>(row_grid<KV_WRITE_ELEMS>, c->head_dim, stream, a) : write_by_dim<DT, KV_BF16, false>(row_grid<KV_WRITE_ELEMS>, c->head_dim, stream, a);
     };
     if (dtype == POCR_F32) return go(std::integral_constant<int, DT_F32>());
     if (dtype == POCR_BF16) return go(std::integral_constant<int, DT_BF16>());
@@ -234,7 +235,7 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *c, const void
     KvReadArgs a{c->k, c->v, c->k_exp, c->v_exp, k, v, slots, c->num_pages, c->kv_heads, page_shift(c), (uint32_t)(tokens * 2 * c->kv_heads), slots64};
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        return c->format == POCR_KV_FP8 ? read_by_dim<DT, KV_FP8>(row_grid, c->head_dim, stream, a) : read_by_dim<DT, KV_BF16>(row_grid, c->head_dim, stream, a);
+        return c->format == POCR_KV_FP8 ? read_by_dim<DT, KV_FP8>(row_grid<KV_READ_ELEMS>, c->head_dim, stream, a) : read_by_dim<DT, KV_BF16>(row_grid<KV_READ_ELEMS>, c->head_dim, stream, a);
     };
     if (dtype == POCR_F32) return go(std::integral_constant<int, DT_F32>());
     if (dtype == POCR_BF16) return go(std::integral_constant<int, DT_BF16>());

@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                     for (int j = 0; j < 4; ++j) q[rt][st][0].u[j] = (q[rt][st][0].u[j] & qkeep) ^ qflip;
                 } else {
                     float x[8];
-                    load8<DT, true>(qr + Block::key_elem(g, st), x);
+                    load_row<DT, true>(qr + Block::key_elem(g, st), x);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] *= csign;
                     split_planes<QP>(x, q[rt][st]);
