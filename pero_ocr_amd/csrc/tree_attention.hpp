@@ -135,7 +135,7 @@ template <int FMT, int D> struct KvBlock {
     static constexpr int VW = VB < 4 ? 1 : VB / 4;
     uint32_t k[2][KW];
     uint32_t v[8][VW];
-    uint32_t ke[2], ve[2];
+    uint32_t ke[2], ve[2];                                   // four keys' exponents: the lane's among them, its own four
 
     // base[h]: row number of key 0 of half h (of row 0 where the page is absent: in bounds, and masked by the caller); the same for the whole
     // wave, so that a lane's part of the address is a constant 32-bit offset
@@ -150,7 +150,7 @@ template <int FMT, int D> struct KvBlock {
 #pragma unroll
                 for (int c = 0; c < KW / 4; ++c) *reinterpret_cast<kv_u32x4 *>(k[h] + 4 * c) = *reinterpret_cast<const kv_u32x4 *>(kb + (i * (D * ES) + g * 16) + c * 64);
             }
-            if constexpr (FMT == KV_FP8) ke[h] = (a.k_exp + base[h])[i];
+            if constexpr (FMT == KV_FP8) ke[h] = *reinterpret_cast<const uint32_t *>(a.k_exp + base[h] + (i & 12));
         }
     }
     __device__ __forceinline__ void load_values(const TreeAttnArgs &a, const int64_t (&base)[2], uint32_t lane) {
@@ -174,10 +174,10 @@ template <int FMT, int D> struct KvBlock {
         }
     }
     // operand of the first product: elements of step st (32 of them) of the keys of half h
-    __device__ __forceinline__ Frag key(int h, int st) const {
+    __device__ __forceinline__ Frag key(int h, int st, uint32_t lane) const {
         Frag f;
         if constexpr (FMT == KV_FP8) {
-            const float s = kv_scale((uint8_t)ke[h]);
+            const float s = __uint_as_float(__builtin_amdgcn_ubfe(ke[h], (lane & 3) * 8, 8) << 23);
 #pragma unroll
             for (int j = 0; j < 2; ++j) { f.u[2 * j] = fp8_pair(k[h][2 * st + j], s, false); f.u[2 * j + 1] = fp8_pair(k[h][2 * st + j], s, true); }
         } else {
@@ -337,6 +337,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
             page_ids(first_block + wave, ids);
             place(first_block + wave, ids, base, there);
             kv.load_keys(a, base, lane);
+            __builtin_amdgcn_sched_barrier(0);                        // (in the loop's order, or its waits would cover both)
             kv.load_values(a, base, lane);
             page_ids(first_block + wave + NW, ids);
         }
@@ -344,10 +345,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 const int32_t key0 = b << 5;
                 int64_t next[2];
                 uint32_t next_there = 0;
-                const bool more = b + NW < end_block;
-                if (more) {
-                    place(b + NW, ids, next, next_there);
-                    page_ids(b + 2 * NW, ids);
+                // (behind the last block it is requested again, from the cache: a load that a branch may skip would have to be waited for with
+                // all younger ones)
+                place(b + NW, ids, next, next_there);
+                page_ids(b + 2 * NW, ids);
+                if (b + NW >= end_block) {
+                    next[0] = base[0];
+                    next[1] = base[1];
                 }
                 const bool edge = there != ~0u || key0 + 31 >= ctx;   // some key is not seen by every row
                 ta_f32x4 sc[RT][2];
@@ -357,13 +361,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 for (int st = 0; st < ST; ++st)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const Frag kf = kv.key(h, st);
+                        const Frag kf = kv.key(h, st, lane);
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                             for (int pl = QP - 1; pl >= 0; --pl) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.b, q[rt][st][pl].b, sc[rt][h], 0, 0, 0);
                     }
-                if (more) kv.load_keys(a, next, lane);
+                kv.load_keys(a, next, lane);
                 float p[RT][8];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -412,7 +416,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                             for (int pl = PP - 1; pl >= 0; --pl)
                                 o[rt][w * TW + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[t].b, pf[rt][pl].b, o[rt][w * TW + t], 0, 0, 0);
                 }
-                if (more) kv.load_values(a, next, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                kv.load_values(a, next, lane);
                 base[0] = next[0];
                 base[1] = next[1];
                 there = next_there;
