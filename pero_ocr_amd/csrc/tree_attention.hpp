@@ -10,8 +10,8 @@
 // lane & 15 and nothing is exchanged between lanes but, now and then, the row maximum:
 //   S^T = K Q^T     lane (row, g = lane / 16) gets the scores of keys 4 g + r and 16 + 4 g + r of the block, r = 0..3
 //   O^T = V^T P^T   takes exactly these eight probabilities as its operand when V^T is fed in the same key order
-// Keys and values go from HBM straight into registers, no LDS and no barrier in the loop.  K: a lane holds a quarter of one key's
-// row (which quarter of each 64 elements is free to choose, Q is laid out to match), so whole lines are read.  V: a lane loads D / 16 neighbouring elements
+// No barrier in the loop: every wave fetches its own keys.  Which elements of K a step of 32 takes is free to choose, Q is laid out to match.  V goes
+// straight into registers: a lane loads D / 16 neighbouring elements
 // of eight keys and transposes them with byte permutes; tile c of the product then is elements c, D/16 + c, 2 D/16 + c, ... and a lane ends up with
 // D / 4 neighbouring outputs of its row.
 // 8-bit codes become bfloat16 exactly, by v_cvt_scalef32 with the key's own power of two.
@@ -91,6 +91,13 @@ __device__ __forceinline__ float row_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// lanes of a wave write and read each other's LDS words in the order of the program (no instruction: LDS serves a wave in order)
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 union Frag { uint32_t u[4]; ta_bf16x8 b; };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -126,31 +133,48 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w, float scale, bool high)
     return r.u;
 }
 
-// A block of 32 keys as a lane holds it: for K its quarter of key (lane & 15) of both 16-key halves, for V D / 16 elements (from lane & 15 on) of
-// the eight keys 4 g + a and 16 + 4 g + a.
+// A block of 32 keys as a lane holds it: for V D / 16 elements (from lane & 15 on) of the eight keys 4 g + a and 16 + 4 g + a.  For K a lane
+// needs its quarter of key (lane & 15) of both 16-key halves.  Fetched like that, every lane of an instruction asks for 16 bytes of another
+// row, and the address unit takes a cycle for each.  With rows of 8 bits that is still the faster way (24 sequences of 4736 keys, 128
+// rows each: 119 us); with bfloat16, twice the pieces, the lanes fetch neighbouring pieces and the block turns in the wave's part of
+// LDS (177 -> 141 us; in 8 bits it would cost 131).
 template <int FMT, int D> struct KvBlock {
     static constexpr int ES = FMT == KV_FP8 ? 1 : 2;
-    static constexpr int KW = D * ES / 16;                   // dwords of a quarter row
-    static constexpr int VB = D * ES / 16;                   // bytes of V a lane holds per key
+    static constexpr bool STAGED = FMT == KV_BF16;
+    static constexpr int RB = D * ES, PR = RB / 16, KI = PR / 2;      // bytes and pieces of a row, pieces of K a lane fetches
+    static constexpr int PITCH = RB + 16, STAGE = STAGED ? 32 * PITCH : 0;         // of the wave's part of LDS (16 rows at one piece: all 64 banks)
+    static constexpr int VB = D * ES / 16;                            // bytes of V a lane holds per key
     static constexpr int VW = VB < 4 ? 1 : VB / 4;
-    uint32_t k[2][KW];
+    kv_u32x4 k[KI];
     uint32_t v[8][VW];
-    uint32_t ke[2], ve[2];                                   // four keys' exponents: the lane's among them, its own four
+    uint32_t ke[2], ve[2];                                            // four keys' exponents: the lane's among them, its own four
 
     // base[h]: row number of key 0 of half h (of row 0 where the page is absent: in bounds, and masked by the caller); the same for the whole
     // wave, so that a lane's part of the address is a constant 32-bit offset
     __device__ __forceinline__ void load_keys(const TreeAttnArgs &a, const int64_t (&base)[2], uint32_t lane) {
+        constexpr int HALF = KI / 2;                                  // pieces of a half
         const uint32_t i = lane & 15, g = lane >> 4;
+        const uint8_t *kb[2] = {static_cast<const uint8_t *>(a.k) + base[0] * RB, static_cast<const uint8_t *>(a.k) + base[1] * RB};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint8_t *kb = static_cast<const uint8_t *>(a.k) + base[h] * (D * ES);
-            if constexpr (KW == 2) {
-                *reinterpret_cast<kv_u32x2 *>(k[h]) = *reinterpret_cast<const kv_u32x2 *>(kb + (i * (D * ES) + g * 8));
-            } else {
+            if constexpr (STAGED) {
 #pragma unroll
-                for (int c = 0; c < KW / 4; ++c) *reinterpret_cast<kv_u32x4 *>(k[h] + 4 * c) = *reinterpret_cast<const kv_u32x4 *>(kb + (i * (D * ES) + g * 16) + c * 64);
+                for (int c = 0; c < HALF; ++c) k[h * HALF + c] = *reinterpret_cast<const kv_u32x4 *>(kb[h] + (c * 64 + lane) * 16);
+            } else {
+                if constexpr (D == 32) *(reinterpret_cast<kv_u32x2 *>(k) + h) = *reinterpret_cast<const kv_u32x2 *>(kb[h] + i * RB + g * 8);
+                else {
+#pragma unroll
+                    for (int c = 0; c < HALF; ++c) k[h * HALF + c] = *reinterpret_cast<const kv_u32x4 *>(kb[h] + (i * RB + g * 16) + c * 64);
+                }
+                ke[h] = *reinterpret_cast<const uint32_t *>(a.k_exp + base[h] + (lane & 12));
             }
-            if constexpr (FMT == KV_FP8) ke[h] = *reinterpret_cast<const uint32_t *>(a.k_exp + base[h] + (i & 12));
+        }
+    }
+    __device__ __forceinline__ void stage_keys(uint8_t *stage, uint32_t lane) const {
+#pragma unroll
+        for (int c = 0; c < KI; ++c) {
+            const uint32_t q = c * 64 + lane;
+            *reinterpret_cast<kv_u32x4 *>(stage + q / PR * PITCH + q % PR * 16) = k[c];
         }
     }
     __device__ __forceinline__ void load_values(const TreeAttnArgs &a, const int64_t (&base)[2], uint32_t lane) {
@@ -173,18 +197,20 @@ template <int FMT, int D> struct KvBlock {
             if constexpr (FMT == KV_FP8) ve[h] = *reinterpret_cast<const uint32_t *>(a.v_exp + base[h] + 4 * g);
         }
     }
-    // operand of the first product: elements of step st (32 of them) of the keys of half h
-    __device__ __forceinline__ Frag key(int h, int st, uint32_t lane) const {
-        Frag f;
-        if constexpr (FMT == KV_FP8) {
-            const float s = __uint_as_float(__builtin_amdgcn_ubfe(ke[h], (lane & 3) * 8, 8) << 23);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) { f.u[2 * j] = fp8_pair(k[h][2 * st + j], s, false); f.u[2 * j + 1] = fp8_pair(k[h][2 * st + j], s, true); }
+    // operands of the first product: steps STEPS * c .. of the keys of half h (a step: 32 elements), from one piece of every key
+    static constexpr int STEPS = D == 32 ? 1 : 2 / ES, PIECES = D / 32 / STEPS;
+    __device__ __forceinline__ void keys(const uint8_t *stage, int h, int c, uint32_t lane, Frag (&f)[STEPS]) const {
+        if constexpr (STAGED) {
+            *reinterpret_cast<kv_u32x4 *>(f[0].u) = *reinterpret_cast<const kv_u32x4 *>(stage + (16 * h + (lane & 15)) * PITCH + (4 * c + (lane >> 4)) * 16);
         } else {
+            const float s = __uint_as_float(__builtin_amdgcn_ubfe(ke[h], (lane & 3) * 8, 8) << 23);
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(k) + 2 * STEPS * (h * PIECES + c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f.u[j] = k[h][4 * st + j];
+            for (int j = 0; j < 2 * STEPS; ++j) {
+                f[j / 2].u[2 * (j & 1)] = fp8_pair(w[j], s, false);
+                f[j / 2].u[2 * (j & 1) + 1] = fp8_pair(w[j], s, true);
+            }
         }
-        return f;
     }
     // element of a row that operand element j of step st stands for
     __device__ static __forceinline__ int key_elem(int g, int st) {
@@ -239,7 +265,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
     const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     constexpr int PITCH = D + 4;                                      // (16 rows, four words each: all 64 banks)
-    __shared__ float osum[NW][RT * 16][PITCH];
+    constexpr int OSUM = NW * RT * 16 * PITCH * 4, STAGES = NW * Block::STAGE;
+    __shared__ __attribute__((aligned(16))) uint8_t memory[OSUM > STAGES ? OSUM : STAGES];     // the waves' keys; behind the loop their sums
+    float (*osum)[RT * 16][PITCH] = reinterpret_cast<float (*)[RT * 16][PITCH]>(memory);
+    uint8_t *stage = memory + wave * Block::STAGE;
     __shared__ float stat[NW][RT * 16][2], whole[RT * 16][2];
     __shared__ int64_t place_of[RT * 16];
 
@@ -348,7 +377,6 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 // (behind the last block it is requested again, from the cache: a load that a branch may skip would have to be waited for with
                 // all younger ones)
                 place(b + NW, ids, next, next_there);
-                page_ids(b + 2 * NW, ids);
                 if (b + NW >= end_block) {
                     next[0] = base[0];
                     next[1] = base[1];
@@ -357,17 +385,27 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 ta_f32x4 sc[RT][2];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
+                if constexpr (Block::STAGED) {
+                    wave_order();
+                    kv.stage_keys(stage, lane);
+                    wave_order();
+                }
 #pragma unroll
-                for (int st = 0; st < ST; ++st)
+                for (int c = 0; c < Block::PIECES; ++c)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const Frag kf = kv.key(h, st, lane);
+                        Frag kf[Block::STEPS];
+                        kv.keys(stage, h, c, lane, kf);
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
+                        for (int st = 0; st < Block::STEPS; ++st)
 #pragma unroll
-                            for (int pl = QP - 1; pl >= 0; --pl) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.b, q[rt][st][pl].b, sc[rt][h], 0, 0, 0);
+                            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                                for (int pl = QP - 1; pl >= 0; --pl)
+                                    sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[st].b, q[rt][c * Block::STEPS + st][pl].b, sc[rt][h], 0, 0, 0);
                     }
                 kv.load_keys(a, next, lane);
+                page_ids(b + 2 * NW, ids);                            // (not earlier: a wait for LDS is one for these too)
                 float p[RT][8];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -465,7 +503,6 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
         for (int rt = 0; rt < RT; ++rt) l[rt] = row_sum(l[rt]);
         // ---- the waves' sums meet in LDS: one maximum per row, then every thread adds its share of the outputs in a fixed order and writes it
         // in whole lines
-        __syncthreads();                                              // (the last rows' sums have been read)
         if (g == 0) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -524,6 +561,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 if (a.lse && d == 0) a.lse[to] = ll == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(ll)) * 0.693147180559945f;
             }
         }
+        __syncthreads();                                              // (the sums have been read: their place is the next rows' keys')
     }
 }
 
