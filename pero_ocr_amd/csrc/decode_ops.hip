@@ -118,9 +118,10 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     p.tiles = (int)std::min<int64_t>((rows + 16 * p.rt - 1) / (16 * p.rt), 1024);
     const int64_t units = pairs * p.tiles, blocks = (((int64_t)t->max_pages << page_shift(c)) + 31) / 32;
     // A workgroup costs about 4 us to start and to end (cold scalar loads, the join of its waves), a block of 32 keys 0.3 us a wave: no split below
-    // 32 blocks (one sequence, 4129 keys, 264 rows: 4 splits 19.9 us, 8 splits 20.5, 16 splits 23.4), and no more workgroups than run at once
-    // (four sequences of 60-131 thousand keys: 256 workgroups 180 us, 512 173 us, 640 191 us, 1024 195 us).
-    p.nsplit = (int)std::max<int64_t>(1, std::min({512 / units, blocks / 32, (int64_t)TA_MAX_SPLITS}));
+    // 32 blocks (one sequence, 4129 keys, 264 rows: 4 splits 19.9 us, 8 splits 20.5, 16 splits 23.4), and no more workgroups than run at once, two
+    // on a CU (four sequences of 60-131 thousand keys: 256 workgroups 186 us, 512 169 us, 768 172 us).  Where sequences have several row tiles
+    // at most, many of them have fewer (8 trees of 10 to 40 tokens: room for 512 workgroups 76 us, for 768 61 us).
+    p.nsplit = (int)std::max<int64_t>(1, std::min({(p.tiles > 1 ? 768 : 512) / units, blocks / 32, (int64_t)TA_MAX_SPLITS}));
     p.waves = p.rt == 1 && units >= 2048 ? 1 : 4;
     p.groups = (pairs * p.nsplit + 7) / 8 * 8 * p.tiles;
     return p;

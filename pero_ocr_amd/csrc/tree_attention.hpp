@@ -25,6 +25,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 #include "kv_cache.hpp"
 
 namespace pocr {
@@ -596,12 +597,25 @@ __global__ __launch_bounds__(256) void tree_attention_join_kernel(TreeAttnArgs a
     }
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
     const float *po = a.part + (int64_t)at * D + (D < 64 ? lane & (D - 1) : lane * E);
-#pragma unroll 8
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float fs = __shfl(s < 64 ? f[0] : f[1], s & 63, 64);
+    auto add = [&](auto width) {                                      // sums on their way at once: a launch of few rows is a chain of round trips
+        constexpr int U = decltype(width)::value;
+        for (int s0 = 0; s0 < a.nsplit; s0 += U) {
+            float x[U][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += fs * po[(int64_t)s * total * D + e];
-    }
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[u][e] = po[(int64_t)min(s0 + u, a.nsplit - 1) * total * D + e];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int s = s0 + u;
+                const float fs = __shfl(s < 64 ? f[0] : f[1], s & 63, 64);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += s < a.nsplit ? fs * x[u][e] : 0.f;
+            }
+        }
+    };
+    if (a.nsplit <= 4) add(std::integral_constant<int, 4>());
+    else add(std::integral_constant<int, 16>());
     T *out = static_cast<T *>(a.out) + (int64_t)at * D + lane * E;
     if (lane * E < D) {
 #pragma unroll

@@ -252,8 +252,8 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
             qs, at = q.stride(), q.data_ptr()
         args = _native.TreeAttentionArgs(
             at, out.data_ptr(), lse.data_ptr() if want_lse else None, page_table.data_ptr(), lengths.data_ptr(), q_start.data_ptr(),
-            mask.data_ptr() if mask is not None else None, None, 0, qs[0], qs[1], ps[0], mask.stride(0) if mask is not None else 0, tokens, max_queries,
-            _DTYPES[q.dtype], seqs, heads, width, mask.shape[1] if mask is not None else 0, fresh, dim ** -0.5 if scale is None else scale)
+            mask.data_ptr() if mask is not None else None, None, 0, qs[0], qs[1], ps[0], mask.stride(0) if mask is not None else 0, tokens, int(max_queries),
+            _DTYPES[q.dtype], seqs, heads, width, mask.shape[1] if mask is not None else 0, fresh, dim ** -0.5 if scale is None else float(scale))
         need = lib.pocr_tree_attention_workspace(n, args)
         if need:
             if need < 0:
@@ -280,6 +280,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     shape = tokens.shape
     if shape[0] != rows or not tokens.is_contiguous():
         raise ValueError(f"tokens: expected a contiguous tensor with {rows} rows, got {tuple(shape)}")
+    top = int(top)
     if classes < 1 or not 0 <= top <= MAX_TOP or top > classes:
         raise ValueError(f"top = {top}: 0 .. {MAX_TOP}, and at most the {classes} classes")
     stride, last = logits.stride()

@@ -444,6 +444,40 @@ def test_gpu_attention_padded_batch():
 
 
 @pytest.mark.gpu
+def test_gpu_attention_in_place_and_without_pages():
+    """the outputs may take the queries' place, split or not; sequences without any page see nothing"""
+    for lengths, counts in (([40, 70], [3, 2]), ([3000, 2100], [3, 2])):
+        p = _problem(lengths, counts, 4, 2, 64, 16, "bf16", "fp8", 45, mask="tree")
+        want = ops.tree_attention(**p)
+        q = p["q"].clone()
+        assert ops.tree_attention(**dict(p, q=q, out=q)) is q and torch.equal(q, want)
+    out, lse = ops.tree_attention(**dict(p, page_table=p["page_table"][:, :0]), want_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    empty = ops.tree_attention(p["q"][:0], p["pages"], p["page_table"][:0], none, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert empty.shape == (0, 4, 64)
+    with pytest.raises(RuntimeError, match="without a sequence"):
+        ops.tree_attention(p["q"], p["pages"], p["page_table"][:0], none, torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_gpu_attention_split_extremes():
+    """sequences of very different lengths that share one cut into splits: empty splits, splits that see nothing, one long sequence"""
+    p = _problem([9000, 1, 33, 2000, 0], [1, 1, 2, 3, 0], 2, 1, 64, 64, "fp32", "fp8", 49, mask="tree", tail=2)
+    p["page_table"][3, 5:20] = -1                                    # 960 positions that are absent
+    _check_dense(p, ops.tree_attention(**p, want_lse=True))
+    p["page_table"][0, :-2] = -1
+    _check_dense(p, ops.tree_attention(**p, want_lse=True))
+
+
+def _check_dense(p, got):
+    """against the oracle on the rows of the sequences; the rows behind them are zeros"""
+    n = int(p["q_start"][-1])
+    _check(dict(p, q=p["q"][:n], mask=p["mask"][:n]), "fp32", [t[:n] for t in got])
+    assert (got[0][n:] == 0).all() and torch.isneginf(got[1][n:]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shift", [0, 1])
 def test_gpu_attention_strided_queries(shift):
     p = _problem([20, 50], [2, 3], 4, 2, 64, 16, "bf16", "fp8", 43)
