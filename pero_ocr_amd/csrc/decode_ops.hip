@@ -78,6 +78,8 @@ int check_pages(const pocr_kv_pages *c) {
 int check_rows(const pocr_kv_pages *c, int64_t tokens, const char *what) {
     if (tokens < 0) return refuse("%s: tokens %lld", what, (long long)tokens);
     if (tokens > ((int64_t)1 << 31) / (2 * (int64_t)c->kv_heads) - 128) return refuse("%s: 2 * tokens * kv_heads must stay below 2^31", what);
+    // (8 elements a thread, and a launch has fewer than 2^32 threads)
+    if (tokens * 2 * c->kv_heads * (c->head_dim / 8) > (int64_t)1 << 31) return refuse("%s: 2 * tokens * kv_heads * head_dim must not exceed 2^34", what);
     return 0;
 }
 
@@ -108,22 +110,35 @@ template <int E> dim3 row_grid(uint32_t rows, int D) { const uint32_t per = 256 
 constexpr bool two_tiles(int dtype, int D) { return D <= 64 || (D == 128 && dtype != POCR_F32); }
 
 // How the work of one attention call is cut.
-struct AttendPlan { int rt, tiles, nsplit, waves; int64_t groups; };
+struct AttendPlan { int rt, tiles, nsplit, waves; int64_t slots, run, groups; };
 
 AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
     AttendPlan p;
-    const int64_t most = t->max_queries > 0 && t->max_queries < t->tokens ? t->max_queries : t->tokens;
-    const int64_t rows = most * (t->heads / c->kv_heads), pairs = (int64_t)t->seqs * c->kv_heads;
-    p.rt = rows > 16 && two_tiles(t->dtype, c->head_dim) ? 2 : 1;
-    p.tiles = (int)std::min<int64_t>((rows + 16 * p.rt - 1) / (16 * p.rt), 1024);
-    const int64_t units = pairs * p.tiles, blocks = (((int64_t)t->max_pages << page_shift(c)) + 31) / 32;
-    // A workgroup costs about 4 us to start and to end (cold scalar loads, the join of its waves), a block of 32 keys 0.3 us a wave: no split below
-    // 32 blocks (one sequence, 4129 keys, 264 rows: 4 splits 19.9 us, 8 splits 20.5, 16 splits 23.4), and no more workgroups than run at once, two
-    // on a CU (four sequences of 60-131 thousand keys: 256 workgroups 186 us, 512 169 us, 768 172 us).  Where sequences have several row tiles
-    // at most, many of them have fewer (8 trees of 10 to 40 tokens: room for 512 workgroups 76 us, for 768 61 us).
-    p.nsplit = (int)std::max<int64_t>(1, std::min({(p.tiles > 1 ? 768 : 512) / units, blocks / 32, (int64_t)TA_MAX_SPLITS}));
+    const int64_t average = (t->tokens + t->seqs - 1) / t->seqs, group = t->heads / c->kv_heads, known = std::min(t->max_queries, t->tokens);
+    p.rt = (known > 0 ? known : average) * group > 16 && two_tiles(t->dtype, c->head_dim) ? 2 : 1;
+    // Slots for row tiles: the same number for each sequence where that is not more than what their rows could need together (then nothing has to
+    // be looked up: 2048 sequences of 8 tokens 510 us, looked up 615 us), or as many as its rows need (8 single tokens next to one of
+    // 512: 81 us, slots for 512 in each 114 us; 256 single tokens of which nobody said so 53 us, slots for all of them in each 295 us).
+    const int64_t all = t->tokens * group / (16 * p.rt), most = known > 0 ? (known * group + 16 * p.rt - 1) / (16 * p.rt) : all + 1;
+    p.tiles = most * t->seqs <= all + t->seqs ? (int)most : 0;
+    p.slots = p.tiles ? p.tiles * (int64_t)t->seqs : all + t->seqs;
+    const int64_t units = (p.tiles ? p.slots : all + (t->seqs + 1) / 2) * c->kv_heads, blocks = (((int64_t)t->max_pages << page_shift(c)) + 31) / 32;
+    // Splits for one workgroup on each CU, of 10 blocks of 32 keys or more: a workgroup costs about 4 us to start and to end (single tokens, 8 key
+    // heads of 128, 4 query heads each; in brackets the rule's: 500 keys [1] 8.6 us, 2 splits 10.0; 2000 keys 1 split 17.3, 3 12.9, [6] 11.4;
+    // 8 sequences of 4000 keys 1 split 29.8, 2 21.8, [4] 19.0, 6 20.6; 32 sequences [1] 47, 2 49).  Two workgroups on each where a split still is
+    // 256 blocks, so that sequences of different lengths end together (60 to 131 thousand keys: 256 workgroups 186 us, 512 169 us, 768 172 us).
+    p.nsplit = (int)std::min<int64_t>({std::max({std::min(256 / units, blocks / 10), std::min(512 / units, blocks / 256), (int64_t)1}), TA_MAX_SPLITS,
+                                       std::max<int64_t>((1 << 26) / (t->tokens * t->heads), 1)});
     p.waves = p.rt == 1 && units >= 2048 ? 1 : 4;
-    p.groups = (pairs * p.nsplit + 7) / 8 * 8 * p.tiles;
+    // Lists of slots: one for every key head and split.  Tiles of a sequence share their XCD's L2 when a list stays on one XCD (24 trees, 128 rows:
+    // 204 us, in runs of 8 slots 227, of 2 292, of 1 375); with lists that 8 XCDs cannot share evenly, in runs of up to 16.
+    const int64_t lists = (int64_t)c->kv_heads * p.nsplit, work = p.slots * lists;
+    p.run = 1;
+    if (p.tiles != 1) {
+        if (lists % 8 == 0) p.run = p.slots;
+        else while (p.run < 16 && work / p.run >= 128) p.run *= 2;
+    }
+    p.groups = (work + 8 * p.run - 1) / (8 * p.run) * (8 * p.run);
     return p;
 }
 
@@ -155,16 +170,21 @@ int check_attention(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
     if (t->heads < 1 || t->heads % c->kv_heads) return refuse("pocr_tree_attention: heads %d must be a multiple of the cache's %d key heads", t->heads, c->kv_heads);
     if (t->max_pages < 0) return refuse("pocr_tree_attention: max_pages %d", t->max_pages);
     if (t->tokens > 0 && t->seqs == 0) return refuse("pocr_tree_attention: tokens without a sequence");
-    if ((int64_t)t->seqs * c->kv_heads > 1 << 20 || t->tokens * t->heads > 0x7fffffff)
-        return refuse("pocr_tree_attention: seqs * kv_heads exceeds 2^20 or tokens * heads 2^31");
+    if ((int64_t)t->seqs * c->kv_heads > 1 << 20 || t->tokens * t->heads > 1 << 27)
+        return refuse("pocr_tree_attention: seqs * kv_heads exceeds 2^20 or tokens * heads 2^27");
     return 0;
 }
+
+// Threads of a row: 16 lanes, a wave, four waves or a workgroup of 1024.
+int score_threads(int classes) { return classes <= 512 ? 16 : classes <= 4096 ? 64 : classes <= 32768 ? 256 : 1024; }
 
 int check_scores(const pocr_token_logprobs_args *t) {
     if (!t) return refuse("pocr_token_logprobs: NULL arguments");
     if (!known_dtype(t->dtype)) return refuse("pocr_token_logprobs: dtype %d", t->dtype);
     if (t->rows < 0 || t->rows > 0x7fffffff) return refuse("pocr_token_logprobs: rows %lld", (long long)t->rows);
     if (t->classes < 1 || t->classes > 1 << 30) return refuse("pocr_token_logprobs: classes %d", t->classes);
+    if (t->rows * score_threads(t->classes) >= (int64_t)1 << 32)        // (a launch has fewer threads)
+        return refuse("pocr_token_logprobs: rows %lld: with %d classes fewer than %lld", (long long)t->rows, t->classes, (1ll << 32) / score_threads(t->classes));
     if (t->given < 0) return refuse("pocr_token_logprobs: given %d", t->given);
     if (t->top < 0 || t->top > LP_MAX_TOP || t->top > t->classes) return refuse("pocr_token_logprobs: top %d must be in 0..%d and at most the classes", t->top, LP_MAX_TOP);
     return 0;
@@ -187,8 +207,9 @@ template <int DT> int score(void *stream, const LogprobArgs &a) {
     const unsigned rows = (unsigned)a.rows;
     if (a.C <= 256) return launch(w, token_logprobs_few_kernel<DT, 16>, dim3((rows + 15) / 16), dim3(256), stream, a);
     if (a.C <= 512) return launch(w, token_logprobs_few_kernel<DT, 32>, dim3((rows + 15) / 16), dim3(256), stream, a);
-    if (a.C <= 4096) return launch(w, token_logprobs_kernel<DT, 64>, dim3(rows), dim3(64), stream, a);
-    if (a.C <= 32768) return launch(w, token_logprobs_kernel<DT, 256>, dim3(rows), dim3(256), stream, a);
+    const int threads = score_threads(a.C);
+    if (threads == 64) return launch(w, token_logprobs_kernel<DT, 64>, dim3(rows), dim3(64), stream, a);
+    if (threads == 256) return launch(w, token_logprobs_kernel<DT, 256>, dim3(rows), dim3(256), stream, a);
     if (a.slices == 1) return launch(w, token_logprobs_kernel<DT, 1024>, dim3(rows), dim3(1024), stream, a);
     if (launch(w, token_logprobs_kernel<DT, 256, true>, dim3(rows * a.slices), dim3(256), stream, a)) return 1;
     return launch(w, token_logprobs_join_kernel<DT>, dim3(rows), dim3(256), stream, a);
@@ -266,7 +287,7 @@ int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, con
     if (dev.enter(device_id)) return 1;
     TreeAttnArgs a{t->q, c->k, c->v, c->k_exp, c->v_exp, t->page_table, t->lengths, t->q_start, t->mask, t->out, t->lse, static_cast<float *>(t->workspace),
                    t->q_token_stride, t->q_head_stride, t->page_table_stride, t->mask_stride, t->tokens, t->seqs, t->heads, c->kv_heads, c->num_pages, page_shift(c),
-                   t->max_pages, t->mask_words, t->zero_rest, p.nsplit, p.tiles, t->scale};
+                   t->max_pages, t->mask_words, t->zero_rest, p.nsplit, p.tiles, (uint32_t)p.slots, (uint32_t)p.run, t->scale};
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         return c->format == POCR_KV_FP8 ? attend_by_dim<DT, KV_FP8>(c->head_dim, p, stream, a) : attend_by_dim<DT, KV_BF16>(c->head_dim, p, stream, a);

@@ -45,6 +45,7 @@ struct TreeAttnArgs {
     float *part;                  // nsplit > 1: sums [nsplit][tokens * heads][D], then (maximum, sum) [nsplit][tokens * heads][2]
     int64_t q_ts, q_hs, table_stride, mask_stride, tokens;
     int32_t seqs, heads, kv_heads, num_pages, page_shift, max_pages, mask_words, zero_rest, nsplit, tiles;
+    uint32_t slots, run;
     float scale;
 };
 
@@ -273,44 +274,60 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
     __shared__ float stat[NW][RT * 16][2], whole[RT * 16][2];
     __shared__ int64_t place_of[RT * 16];
 
-    // workgroups that read the same keys (the row tiles of one sequence, key head and split) are 8 apart: consecutive workgroups go to
-    // different XCDs, so these share an L2
-    const uint32_t lane8 = blockIdx.x & 7, rest8 = blockIdx.x >> 3, tile0 = rest8 % (uint32_t)a.tiles;
-    const uint32_t stream = (rest8 / (uint32_t)a.tiles) * 8 + lane8, pairs = (uint32_t)a.seqs * a.kv_heads;
-    if (stream >= pairs * (uint32_t)a.nsplit) return;
-    const int split = (int)(stream / pairs), pair = (int)(stream - split * pairs), s = pair / a.kv_heads, hk = pair - s * a.kv_heads;
+    if (a.zero_rest) {                                                // rows of no sequence, a share for every workgroup
+        const int32_t end = min(max(((ScalarInts)a.starts)[a.seqs], 0), (int32_t)a.tokens);
+        const int64_t from = (int64_t)end * a.heads, rest = (a.tokens - end) * a.heads, all = (int64_t)gridDim.x * (64 * NW);
+        constexpr int PIECES = D * sizeof(T) / 16;
+        for (int64_t p = (int64_t)blockIdx.x * (64 * NW) + tid; p < rest * PIECES; p += all) static_cast<kv_u32x4 *>(a.out)[from * PIECES + p] = (kv_u32x4){0, 0, 0, 0};
+        if (a.lse)
+            for (int64_t p = (int64_t)blockIdx.x * (64 * NW) + tid; p < rest; p += all) a.lse[from + p] = -INFINITY;
+    }
+
+    // Consecutive workgroups go to different XCDs; runs of `run` slots stay on one, so that the row tiles of one sequence and key head, which
+    // read the same keys, share an L2.  With one tile a sequence, key heads are next to each other instead: no XCD has a long sequence to itself.
+    const uint32_t turn = (blockIdx.x >> 3) / a.run, number = (turn * 8 + (blockIdx.x & 7)) * a.run + ((blockIdx.x >> 3) - turn * a.run);
+    const uint32_t group = (uint32_t)a.heads / (uint32_t)a.kv_heads, pairs = a.slots * (uint32_t)a.kv_heads;
+    const int split = (int)(number / pairs);
+    const uint32_t pair = number - (uint32_t)split * pairs, slot = a.tiles == 1 ? pair / (uint32_t)a.kv_heads : pair % a.slots;
+    const int hk = (int)(a.tiles == 1 ? pair - slot * (uint32_t)a.kv_heads : pair / a.slots);
+    if (split >= a.nsplit) return;
+    // Slots: `tiles` for each sequence, or (tiles = 0) as many as its rows need: sequence s then begins at slot_of(first row), which leaves it
+    // one more than its whole tiles.
+    auto slot_of = [&](int32_t first, int i) { return (uint32_t)min(max(first, 0), (int32_t)a.tokens) * group / (16 * RT) + (uint32_t)i; };
+    int s = 0;
+    if (a.tiles) s = (int)(slot / (uint32_t)a.tiles);
+    else {
+        int left = a.seqs;
+        while (left > 1) {                                            // the last sequence that begins at or before this slot: 64 looked at in a step
+            const int step = (left + 63) / 64, at = s + min(lane * step, left - 1);
+            const int n = (int)__popcll(__ballot(lane * step < left && slot_of(a.starts[at], at) <= slot)), skip = max(n - 1, 0) * step;
+            s += skip;
+            left = min(step, left - skip);
+        }
+        s = __builtin_amdgcn_readfirstlane(s);
+    }
     const TreeSeq sq = tree_seq(a, s);
-    const int group = a.heads / a.kv_heads;
-    const uint32_t rows = (uint32_t)sq.n * (uint32_t)group;           // (tokens * heads < 2^31)
+    const uint32_t rows = (uint32_t)sq.n * group, tile0 = slot - (a.tiles ? (uint32_t)(s * a.tiles) : slot_of(sq.first, s));
+    if (tile0 >= (rows + 16 * RT - 1) / (16 * RT)) return;            // an unused slot, or a sequence without new tokens
     const int32_t *table = a.table + s * a.table_stride;
     // scores in units of log2: the sign of the scale goes to the query, so that the largest product is the largest score; 0 makes the query 0
     const float c = a.scale * 1.44269504088896f;
     const float csign = c == 0.f ? 0.f : c < 0.f ? -1.f : 1.f, cabs = c == 0.f ? 1.f : fabsf(c);
     const uint32_t qkeep = c == 0.f ? 0u : ~0u, qflip = c < 0.f ? 0x80008000u : 0u;          // the same for bfloat16 queries, on the bits
 
-    if (a.zero_rest && s == a.seqs - 1 && split == 0) {               // rows of no sequence
-        const uint32_t rest = ((uint32_t)a.tokens - (uint32_t)(sq.first + sq.n)) * (uint32_t)group;
-        for (uint32_t r = tile0 * (64 * NW) + tid; r < rest; r += (uint32_t)a.tiles * (64 * NW)) {
-            const int64_t at = (int64_t)(sq.first + sq.n + (int32_t)(r / group)) * a.heads + hk * group + (int32_t)(r % group);
-#pragma unroll 1
-            for (int d = 0; d < D; ++d) static_cast<T *>(a.out)[at * D + d] = (T)0.f;
-            if (a.lse) a.lse[at] = -INFINITY;
-        }
-    }
-
     const int32_t blocks = (int32_t)(((uint32_t)sq.len + 31u) >> 5), per = (int32_t)(((uint32_t)blocks + a.nsplit - 1u) / (uint32_t)a.nsplit);
     const int32_t first_block = min(split * per, blocks), end_block = min(first_block + per, blocks);
     const int32_t ctx = sq.len - sq.n;
 
-    for (uint32_t r0 = tile0 * (16 * RT); r0 < rows; r0 += (uint32_t)a.tiles * (16 * RT)) {
+    for (uint32_t r0 = tile0 * (16 * RT); r0 < rows; r0 += a.tiles ? (uint32_t)a.tiles * (16 * RT) : rows) {
         int32_t tok[RT];
         int64_t at[RT];                                               // row of out, -1: none
         Frag q[RT][ST][QP];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const uint32_t r = r0 + 16 * rt + row, rr = min(r, rows - 1);
-            tok[rt] = (int32_t)(rr / (uint32_t)group);
-            const int head = hk * group + (int)(rr - (uint32_t)tok[rt] * (uint32_t)group);
+            tok[rt] = (int32_t)(rr / group);
+            const int head = hk * (int)group + (int)(rr - (uint32_t)tok[rt] * group);
             at[rt] = r < rows ? (int64_t)(sq.first + tok[rt]) * a.heads + head : -1;
             const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + head * a.q_hs;
 #pragma unroll
@@ -476,7 +493,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
 #pragma unroll
                 for (int t = 0; t < NB; ++t) o[rt][t] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
                 const uint32_t rr = min(r0 + 16 * rt + row, rows - 1);
-                const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + (hk * group + (int)(rr - (uint32_t)tok[rt] * (uint32_t)group)) * a.q_hs;
+                const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + (hk * (int)group + (int)(rr - (uint32_t)tok[rt] * group)) * a.q_hs;
                 for (int32_t b = first_block + wave; b < end_block; b += NW)
                     for (int32_t key = b << 5, n = min(32, sq.len - key); n > 0; --n, ++key) {
                         const int64_t kr = kv_row_base(table, a.max_pages, a.num_pages, a.kv_heads, hk, a.page_shift, key);

@@ -80,6 +80,25 @@ def test_c_entries_refuse_bad_arguments():
         assert lib.pocr_tree_attention(0, None, pages, args) == 1 and "workspace" in _err()
 
 
+def test_c_entries_refuse_more_work_than_a_launch_holds():
+    """a grid has fewer than 2^32 threads: said before anything is enqueued"""
+    lib, p = _native.load(), 1 << 20
+    wide = _fake_pages(head_dim=256)
+    for tokens, ok in ((1 << 24, True), ((1 << 24) + 1, False)):           # 2^26 rows of 32 threads
+        rows = _native.KvRows(None, p, p, 512, 256, 512, 256, tokens, 1, 1)
+        assert lib.pocr_kv_write(0, None, wide, rows) == 1 and ("NULL" if ok else "head_dim") in _err()
+        assert lib.pocr_kv_read(0, None, wide, p, 1, tokens, None, p, 1) == 1 and ("NULL" if ok else "head_dim") in _err()
+    args = _native.TreeAttentionArgs(q=None, out=p, page_table=p, lengths=p, q_start=p, tokens=1 << 26, seqs=4, heads=2, max_pages=1, q_head_stride=64, q_token_stride=128)
+    assert lib.pocr_tree_attention(0, None, _fake_pages(), args) == 1 and "NULL" in _err()
+    args.tokens += 1
+    assert lib.pocr_tree_attention(0, None, _fake_pages(), args) == 1 and "2^27" in _err()
+    for classes, rows in ((512, 1 << 28), (4096, 1 << 26), (32768, 1 << 24), (32769, 1 << 22)):
+        args = _native.TokenLogprobsArgs(logits=None, tokens=p, logprob=p, entropy=p, top_logprob=p, top_index=p, row_stride=classes, rows=rows - 16, classes=classes, given=1)
+        assert lib.pocr_token_logprobs(0, None, args) == 1 and "NULL" in _err()
+        args.rows = rows
+        assert lib.pocr_token_logprobs(0, None, args) == 1 and "rows" in _err()
+
+
 def test_python_refusals_on_cpu_tensors():
     k = torch.zeros(2, 2, 16, 64, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="no CPU path"):
@@ -441,6 +460,47 @@ def test_gpu_attention_padded_batch():
     same = ops.tree_attention(**p, out=given)
     assert same is given and (given[5:] == 7).all() and torch.equal(given[:5], out[:5])
     _check(p, "bf16", (out, lse))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads", [1, 3, 8])
+@pytest.mark.parametrize("seqs", [1, 2, 63, 65, 300])
+def test_gpu_attention_ragged_batches(seqs, kv_heads):
+    """every row of a ragged batch is somebody's, whatever the caller says of the longest sequence, and the rows behind the last one are zeros"""
+    rng = np.random.RandomState(seqs)
+    counts = [int(rng.choice([0, 0, 1, 1, 2, 3, 9])) for _ in range(seqs)]
+    counts[seqs // 2] = 41
+    lengths = [n + int(rng.randint(0, 60)) for n in counts]
+    p = _problem(lengths, counts, 4 * kv_heads, kv_heads, 32, 16, "fp32", "bf16", seqs + kv_heads, mask="tree", tail=70)
+    for most in (0, 1, 41, 10 ** 6):
+        _check_dense(p, ops.tree_attention(**p, max_queries=most, want_lse=True))
+
+
+@pytest.mark.gpu
+def test_gpu_attention_thousands_of_sequences():
+    """more sequences than one step of the search tells apart twice over, of lengths that nobody names; most of them are empty"""
+    seqs, rng = 5000, np.random.RandomState(7)
+    counts = [0] * seqs
+    for s in rng.choice(seqs, 90, replace=False):
+        counts[s] = int(rng.randint(1, 12))
+    counts[0] = counts[-1] = 3
+    lengths = [n + (int(rng.randint(0, 20)) if n else 0) for n in counts]
+    p = _problem(lengths, counts, 16, 8, 32, 16, "fp32", "fp8", 71, mask="tree", tail=3)
+    for most in (0, 1, 11):
+        _check_dense(p, ops.tree_attention(**p, max_queries=most, want_lse=True))
+
+
+@pytest.mark.gpu
+def test_gpu_attention_many_tokens_without_a_hint():
+    """2100 sequences of 8 tokens: rows and workgroups by the rows that there are (every sequence has room for all tokens: a launch that HIP refuses)"""
+    seqs = 2100
+    p = _problem([16] * seqs, [8] * seqs, 64, 8, 32, 16, "bf16", "fp8", 72)
+    out = ops.tree_attention(**p)
+    assert torch.equal(out, ops.tree_attention(**p, max_queries=8))
+    few = dict(p, q=p["q"][:24].clone(), page_table=p["page_table"][:3], lengths=p["lengths"][:3], q_start=p["q_start"][:4])
+    got = ops.tree_attention(**few, want_lse=True)
+    _check(few, "bf16", got)
+    assert torch.equal(got[0], out[:24])
 
 
 @pytest.mark.gpu
