@@ -175,16 +175,16 @@ int check_attention(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
     return 0;
 }
 
-// Threads of a row: 16 lanes, a wave, four waves or a workgroup of 1024.
-int score_threads(int classes) { return classes <= 512 ? 16 : classes <= 4096 ? 64 : classes <= 32768 ? 256 : 1024; }
+// Rows of one call: HIP's limit of 2^32 threads to a launch, for what a row of so many classes may take.
+int64_t score_rows(int classes) { return ((int64_t)1 << 32) / (classes <= 512 ? 16 : classes <= 4096 ? 64 : classes <= 32768 ? 256 : 1024); }
 
 int check_scores(const pocr_token_logprobs_args *t) {
     if (!t) return refuse("pocr_token_logprobs: NULL arguments");
     if (!known_dtype(t->dtype)) return refuse("pocr_token_logprobs: dtype %d", t->dtype);
     if (t->rows < 0 || t->rows > 0x7fffffff) return refuse("pocr_token_logprobs: rows %lld", (long long)t->rows);
     if (t->classes < 1 || t->classes > 1 << 30) return refuse("pocr_token_logprobs: classes %d", t->classes);
-    if (t->rows * score_threads(t->classes) >= (int64_t)1 << 32)        // (a launch has fewer threads)
-        return refuse("pocr_token_logprobs: rows %lld: with %d classes fewer than %lld", (long long)t->rows, t->classes, (1ll << 32) / score_threads(t->classes));
+    if (t->rows >= score_rows(t->classes))
+        return refuse("pocr_token_logprobs: rows %lld: with %d classes fewer than %lld", (long long)t->rows, t->classes, (long long)score_rows(t->classes));
     if (t->given < 0) return refuse("pocr_token_logprobs: given %d", t->given);
     if (t->top < 0 || t->top > LP_MAX_TOP || t->top > t->classes) return refuse("pocr_token_logprobs: top %d must be in 0..%d and at most the classes", t->top, LP_MAX_TOP);
     return 0;
@@ -202,17 +202,29 @@ int64_t score_workspace(const pocr_token_logprobs_args *t) {
     return parts == t->rows ? 0 : parts * (16 + 8 * (int64_t)t->top);
 }
 
+// Few classes in registers: 16 lanes a row where there are rows enough for every SIMD (36864 rows of 232 in fp32, top 4: 12.3 us, with 64 lanes
+// 23.9), 64 lanes where not (600 rows: 4.1 us, with 16 4.8; even at 2400).  An alternative costs a pass over the registers, so above 256 classes only
+// to 8 of them (500 classes, fp32: top 4 22.7 us against 33.5 by a wave that looks among the largest, top 8 32 and 35, top 20 62 and 47), and
+// with 16-bit logits, whose single loads are half as wide, only for few rows (500 classes, top 8: 48 us against 39).
+// Otherwise a wave (rows enough, and a row too short for more: 2000 classes in fp32, top 4 86 us, with 256 threads 110; 4000 classes 170 and
+// 156), 256 threads (600 rows of 1000 classes, top 20: 7.2 us, a wave 12.1), or 1024 (1024 rows of 131072 in bf16, top 20: 52.7 us, with 256
+// 67.3; 3000 rows of 32000 68.5 and 52.6).
 template <int DT> int score(void *stream, const LogprobArgs &a) {
     const char *w = "pocr_token_logprobs";
-    const unsigned rows = (unsigned)a.rows;
-    if (a.C <= 256) return launch(w, token_logprobs_few_kernel<DT, 16>, dim3((rows + 15) / 16), dim3(256), stream, a);
-    if (a.C <= 512) return launch(w, token_logprobs_few_kernel<DT, 32>, dim3((rows + 15) / 16), dim3(256), stream, a);
-    const int threads = score_threads(a.C);
-    if (threads == 64) return launch(w, token_logprobs_kernel<DT, 64>, dim3(rows), dim3(64), stream, a);
-    if (threads == 256) return launch(w, token_logprobs_kernel<DT, 256>, dim3(rows), dim3(256), stream, a);
-    if (a.slices == 1) return launch(w, token_logprobs_kernel<DT, 1024>, dim3(rows), dim3(1024), stream, a);
-    if (launch(w, token_logprobs_kernel<DT, 256, true>, dim3(rows * a.slices), dim3(256), stream, a)) return 1;
-    return launch(w, token_logprobs_join_kernel<DT>, dim3(rows), dim3(256), stream, a);
+    const int64_t rows = a.rows;
+    auto few = [&](void (*kernel)(LogprobArgs), int lanes) { return launch(w, kernel, dim3((unsigned)((rows * lanes + 255) / 256)), dim3(256), stream, a); };
+    auto row = [&](void (*kernel)(LogprobArgs), int threads) {
+        return launch(w, kernel, dim3((unsigned)std::min<int64_t>(rows, LP_GRID), (unsigned)((rows + LP_GRID - 1) / LP_GRID)), dim3(threads), stream, a);
+    };
+    if (a.C <= 256) return rows > 2048 ? few(token_logprobs_few_kernel<DT, 16, 16>, 16) : few(token_logprobs_few_kernel<DT, 64, 4>, 64);
+    if (a.C <= 1024 && a.top <= 8 && rows <= 4096) return a.C <= 512 ? few(token_logprobs_few_kernel<DT, 64, 8>, 64) : few(token_logprobs_few_kernel<DT, 64, 16>, 64);
+    if constexpr (DT == DT_F32)
+        if (a.C <= 512 && a.top <= 8) return few(token_logprobs_few_kernel<DT, 16, 32>, 16);
+    if (a.C <= 2048 && rows > 2048) return row(token_logprobs_kernel<DT, 64>, 64);
+    if (a.C <= 32768) return row(token_logprobs_kernel<DT, 256>, 256);
+    if (a.slices == 1) return row(token_logprobs_kernel<DT, 1024>, 1024);
+    if (launch(w, token_logprobs_kernel<DT, 256, true>, dim3((unsigned)(rows * a.slices)), dim3(256), stream, a)) return 1;
+    return launch(w, token_logprobs_join_kernel<DT>, dim3((unsigned)rows), dim3(256), stream, a);
 }
 
 }  // namespace

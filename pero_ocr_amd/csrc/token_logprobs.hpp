@@ -40,25 +40,31 @@ __device__ __forceinline__ float lp_value(uint32_t key) {
 }
 
 
-// ---- few classes: 16 lanes per row, NV logits in a lane's registers (class lane + 16 i), four rows per wave, so that a reduction of four
-// steps serves four rows.  The alternatives are picked one after the other: the largest key, then the lowest class that has it.
-__device__ __forceinline__ uint32_t max16(uint32_t x) {
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));       // row_ror:8, 4, 2, 1: within 16 lanes
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
-    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
+// ---- few classes: G lanes per row (16: four rows per wave, so that a reduction of four steps serves four rows; or 64), NV logits in a lane's registers
+// (class lane + G i).  The alternatives are picked one after the other: the largest key, then the lowest class that has it.  Bound by the vector
+// unit: 36864 rows of 232 in fp32 with 4 alternatives 12.3 us = 2.9 TB/s, without any 7.5 us = 4.7 TB/s (1.2 us an alternative).
+template <int CTRL> __device__ __forceinline__ uint32_t lp_turn(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, false); }
+
+// the same value in all G lanes: by rotations within 16 lanes, then by exchanging the halves and quarters of the wave
+template <int G, class Op> __device__ __forceinline__ uint32_t lp_all(uint32_t x, Op op) {
+    x = op(x, lp_turn<0x128>(x));                               // row_ror:8, 4, 2, 1
+    x = op(x, lp_turn<0x124>(x));
+    x = op(x, lp_turn<0x122>(x));
+    x = op(x, lp_turn<0x121>(x));
+    if constexpr (G == 64) {
+        const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        x = op((uint32_t)h[0], (uint32_t)h[1]);
+        const auto q = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        x = op((uint32_t)q[0], (uint32_t)q[1]);
+    }
+    return x;
 }
-__device__ __forceinline__ float max16(float x) {
-    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false)));
-    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false)));
-    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, false)));
-    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, false)));
+template <int G> __device__ __forceinline__ uint32_t lp_max(uint32_t x) { return lp_all<G>(x, [](uint32_t a, uint32_t b) { return max(a, b); }); }
+template <int G> __device__ __forceinline__ float lp_max(float x) {
+    return __uint_as_float(lp_all<G>(__float_as_uint(x), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
 }
-__device__ __forceinline__ float sum16(float x) {
-    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
-    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false));
-    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, false));
-    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, false));
+template <int G> __device__ __forceinline__ float lp_sum(float x) {
+    return __uint_as_float(lp_all<G>(__float_as_uint(x), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 
 __device__ __forceinline__ void lp_given(const LogprobArgs &a, int64_t r, int first, int step, float base, float logz, bool none) {
@@ -76,23 +82,23 @@ __device__ __forceinline__ void lp_given(const LogprobArgs &a, int64_t r, int fi
     }
 }
 
-template <int DT, int NV>
+template <int DT, int G, int NV>
 __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) {
     using T = typename ElemOf<DT>::type;
-    const int lane = threadIdx.x & 15;
-    const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (r >= a.rows) return;                                    // (whole groups of 16 lanes)
+    const int lane = threadIdx.x & (G - 1);
+    const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (r >= a.rows) return;                                    // (whole groups of G lanes)
     const T *x = static_cast<const T *>(a.x) + r * a.stride;
     float v[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         v[i] = -INFINITY;
-        if (16 * i + 16 <= a.C || lane + 16 * i < a.C) v[i] = (float)x[lane + 16 * i];
+        if (G * i + G <= a.C || lane + G * i < a.C) v[i] = (float)x[lane + G * i];
     }
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < NV; ++i) m = fmaxf(m, v[i]);
-    m = max16(m);
+    m = lp_max<G>(m);
     const float base = m == -INFINITY ? 0.f : m;
     float z = 0.f, e = 0.f;
 #pragma unroll
@@ -101,12 +107,12 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
         z += p;
         e = fmaf(p, fmaxf(d, -200.f), e);                       // (p is 0 from -104 on)
     }
-    z = sum16(z);
-    e = sum16(e);
+    z = lp_sum<G>(z);
+    e = lp_sum<G>(e);
     const bool none = z == 0.f;
     const float logz = __builtin_amdgcn_logf(z) * 0.693147180559945f;
     if (lane == 0) a.entropy[r] = none ? 0.f : logz - e / z;
-    lp_given(a, r, lane, 16, base, logz, none);
+    lp_given(a, r, lane, G, base, logz, none);
     float *top_lp = a.top_logprob + r * a.top;
     int32_t *top_at = a.top_index + r * a.top;
     // ---- the alternatives: rows of ordinary numbers by the numbers themselves, a taken one becomes -inf
@@ -117,13 +123,13 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
             best = v[0];
 #pragma unroll
             for (int i = 1; i < NV; ++i) best = fmaxf(best, v[i]);
-            best = max16(best);
+            best = lp_max<G>(best);
             if (__ballot(best == -INFINITY)) { plain = false; break; }          // fewer numbers than alternatives
         }
         int slot = NV;
 #pragma unroll
         for (int i = NV - 1; i >= 0; --i) slot = v[i] == best ? i : slot;
-        const uint32_t mine = slot == NV ? 0u : ~(uint32_t)(lane + 16 * slot), low = max16(mine);          // ~class: the largest is the lowest class
+        const uint32_t mine = slot == NV ? 0u : ~(uint32_t)(lane + G * slot), low = lp_max<G>(mine);          // ~class: the largest is the lowest class
         slot = mine == low ? slot : NV;
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = slot == i ? -INFINITY : v[i];
@@ -136,17 +142,17 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
     // rows with NaN or infinities, or with fewer numbers than alternatives: by integer keys
     uint32_t key[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) key[i] = lane + 16 * i < a.C ? lp_key((float)x[lane + 16 * i]) : 0u;          // (below the key of -inf)
+    for (int i = 0; i < NV; ++i) key[i] = lane + G * i < a.C ? lp_key((float)x[lane + G * i]) : 0u;          // (below the key of -inf)
     for (int t = 0; t < a.top; ++t) {
         uint32_t most = 0, low = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) most = max(most, key[i]);
-        most = max16(most);
+        most = lp_max<G>(most);
 #pragma unroll
-        for (int i = NV - 1; i >= 0; --i) low = key[i] == most ? ~(uint32_t)(lane + 16 * i) : low;
-        low = max16(low);
+        for (int i = NV - 1; i >= 0; --i) low = key[i] == most ? ~(uint32_t)(lane + G * i) : low;
+        low = lp_max<G>(low);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = ~low == (uint32_t)(lane + 16 * i) ? 0u : key[i];
+        for (int i = 0; i < NV; ++i) key[i] = ~low == (uint32_t)(lane + G * i) ? 0u : key[i];
         if (lane == 0) {
             top_lp[t] = none ? -INFINITY : (lp_value(most) - base) - logz;
             top_at[t] = (int32_t)~low;
@@ -154,19 +160,25 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
     }
 }
 
-// ---- many classes: a workgroup of B threads per row, one pass over it in 16-byte pieces; thread t takes pieces t, t + B, ... and keeps the
+// ---- many classes: a workgroup of B threads per row, one pass over it in pieces of 16 bytes; thread t takes pieces t, t + B, ... and keeps the
 // running maximum, sum and weighted sum of its own.  The alternatives cost no second pass: a row's k best lie with the threads whose
 // own maximum is among the k largest, so only these threads' pieces (k of B shares) are read again, and of them only what reaches the k-th
 // largest maximum T is kept and ranked.  Where many threads share T (equal logits, rows that are masked but for a few classes) the
 // numbers above T are kept and the lowest classes equal to T are found by reading the row from its start.  What does not fit
 // the list of candidates, and rows with NaN or +inf, take one pass per alternative.
 // Few long rows are cut into slices, a workgroup each (SPLIT), whose sums and alternatives the kernel below joins.
-constexpr int LP_CAND = 1024, LP_SLACK = 32;
+//
+// Bound by HBM where rows are long (1024 rows of 131072 in bf16, top 20: 52.7 us = 5.1 TB/s; 9 rows of 151003 in fp32, which 9 CUs read: 16.5 us, 36
+// GB/s a CU); where they are short by the choice of the alternatives, which a wave makes alone (36864 rows of 1000 in fp32: none 30.5 us, top 4 47.5,
+// top 20 64).  So reductions stay in registers, and the list of a single wave is short: 2.6 KB of LDS let 32 of them share a CU (with 9 KB 17,
+// 52 -> 33 us for rows of 500, top 4).
+constexpr int LP_CAND = 1024, LP_SLACK = 32, LP_GRID = 1 << 21;       // (rows in the first axis of the grid)
+constexpr int lp_cand(int threads) { return threads == 64 ? 256 : LP_CAND; }
 
 template <int DT, int V> __device__ __forceinline__ void lp_load(const void *p, float (&x)[V]) {
     using T = typename ElemOf<DT>::type;
     alignas(16) T t[V];
-    *reinterpret_cast<kv_u32x4 *>(t) = *static_cast<const kv_u32x4 *>(p);
+    __builtin_memcpy(t, static_cast<const T *>(p), 16);         // one load, aligned to an element or better
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] = (float)t[i];
 }
@@ -174,22 +186,21 @@ template <int DT, int V> __device__ __forceinline__ void lp_load(const void *p, 
 template <int DT, int B, bool SPLIT = false>
 __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     using T = typename ElemOf<DT>::type;
-    constexpr int V = 16 / sizeof(T), W = B / 64, U = 4;
-    static_assert(B <= LP_CAND && LP_MAX_TOP <= B, "the list of candidates; a maximum per thread for every alternative");
+    constexpr int V = 16 / sizeof(T), W = B / 64, U = 4, CAND = lp_cand(B);
+    static_assert(B <= CAND && LP_MAX_TOP <= B, "the list of candidates; a maximum per thread for every alternative");
     __shared__ float red[3][W];
     __shared__ uint32_t maxima[B];
     __shared__ uint32_t picked[B];                              // threads whose pieces are read again
-    __shared__ unsigned long long cand[LP_CAND + LP_MAX_TOP];
+    __shared__ unsigned long long cand[CAND + LP_MAX_TOP];
     __shared__ uint32_t limit[2];
     __shared__ int count[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = SPLIT ? blockIdx.x / (uint32_t)a.slices : blockIdx.x;
+    const int64_t r = SPLIT ? blockIdx.x / (uint32_t)a.slices : blockIdx.x + (int64_t)blockIdx.y * LP_GRID;
+    if (r >= a.rows) return;
     const int class0 = SPLIT ? (int)(blockIdx.x - (uint32_t)r * (uint32_t)a.slices) * a.slice : 0, C = SPLIT ? min(a.slice, a.C - class0) : a.C;
     const T *x = static_cast<const T *>(a.x) + r * a.stride + class0;
-    // head elements up to a multiple of 16 bytes, pieces, tail
-    const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
-    const int head = min(off ? V - off : 0, C), pieces = (C - head) / V, tail = C - head - pieces * V;
-    const T *body = x + head;
+    // pieces from the row's start, wherever that lies: which thread sums what, and so the last bit, is not a matter of the address
+    const int pieces = C / V, tail = C - pieces * V;
 
     float m = -INFINITY, ref = 0.f, z = 0.f, e = 0.f;
     auto add = [&](float v) {
@@ -209,7 +220,7 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     for (; i + (U - 1) * B < pieces; i += U * B) {
         float v[U][V];
 #pragma unroll
-        for (int u = 0; u < U; ++u) lp_load<DT, V>(body + (int64_t)(i + u * B) * V, v[u]);
+        for (int u = 0; u < U; ++u) lp_load<DT, V>(x + (int64_t)(i + u * B) * V, v[u]);
         float mx = v[0][0];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -223,7 +234,7 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     }
     for (; i < pieces; i += B) {
         float v[V];
-        lp_load<DT, V>(body + (int64_t)i * V, v);
+        lp_load<DT, V>(x + (int64_t)i * V, v);
         float mx = v[0];
 #pragma unroll
         for (int j = 1; j < V; ++j) mx = fmaxf(mx, v[j]);
@@ -231,11 +242,10 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) add(v[j]);
     }
-    if (tid < head) { const float v = (float)x[tid]; raise(v); add(v); }
-    if (tid < tail) { const float v = (float)body[pieces * V + tid]; raise(v); add(v); }
+    if (tid < tail) { const float v = (float)x[pieces * V + tid]; raise(v); add(v); }
     const float mine = m;
     // ---- the row's maximum and sums
-    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    m = lp_max<64>(m);
     if (lane == 0) red[0][wave] = m;
     __syncthreads();
     for (int w = 0; w < W; ++w) m = fmaxf(m, red[0][w]);
@@ -244,7 +254,8 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
         e = f == 0.f && z == z ? 0.f : f * fmaf(s, z, e);       // (a NaN sum stays one)
         z *= f;
     }
-    for (int o = 32; o >= 1; o >>= 1) { z += __shfl_xor(z, o, 64); e += __shfl_xor(e, o, 64); }
+    z = lp_sum<64>(z);
+    e = lp_sum<64>(e);
     if (lane == 0) { red[1][wave] = z; red[2][wave] = e; }
     if (a.top > 0) maxima[tid] = lp_key(mine);                  // (-inf where a thread has nothing: never among the k best of a larger set)
     if (tid < 2) count[tid] = 0;
@@ -278,7 +289,7 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
             uint32_t mk[W], lo = ~0u;
 #pragma unroll
             for (int w = 0; w < W; ++w) { mk[w] = maxima[w * 64 + lane]; lo = min(lo, mk[w]); }
-            for (int o = 32; o >= 1; o >>= 1) lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
+            lo = ~lp_max<64>(~lo);
             uint32_t hi = lp_key(m) + 1;                        // reached by nobody; lo by all B >= k
             lo = __builtin_amdgcn_readfirstlane(lo);
             hi = __builtin_amdgcn_readfirstlane(hi);
@@ -303,26 +314,25 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
             const uint32_t key = lp_key(v);
             if (key >= from) {
                 const int at = atomicAdd(&count[1], 1);
-                if (at < LP_CAND) cand[at] = (unsigned long long)key << 32 | (uint32_t)~c;
+                if (at < CAND) cand[at] = (unsigned long long)key << 32 | (uint32_t)~c;
             }
         };
         for (int64_t j = tid; j < (int64_t)n_picked * per; j += B) {
             const int piece = (int)(j % per) * B + (int)picked[j / per];
             if (piece < pieces) {
                 float v[V];
-                lp_load<DT, V>(body + (int64_t)piece * V, v);
+                lp_load<DT, V>(x + (int64_t)piece * V, v);
 #pragma unroll
-                for (int q = 0; q < V; ++q) keep(v[q], head + piece * V + q);
+                for (int q = 0; q < V; ++q) keep(v[q], piece * V + q);
             }
         }
         for (int j = tid; j < n_picked; j += B) {
             const int t = (int)picked[j];
-            if (t < head) keep((float)x[t], t);
-            if (t < tail) keep((float)body[pieces * V + t], head + pieces * V + t);
+            if (t < tail) keep((float)x[pieces * V + t], pieces * V + t);
         }
         __syncthreads();
         int n = count[1];
-        bool fits = n <= LP_CAND;
+        bool fits = n <= CAND;
         if (ties && n < k) {                                    // the lowest classes equal to T0 make up the rest
             __syncthreads();
             for (int c0 = 0; c0 < C && n < k; c0 += B) {

@@ -709,6 +709,51 @@ def test_gpu_logprobs_many_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("classes", [5, 63, 256, 257, 300, 512, 1500, 2047])
+def test_gpu_logprobs_special_rows_among_many(classes, kind):
+    """the same special rows where rows are many (other kernels than for few): each block of 16 answers as the first"""
+    low, g = torch.finfo(TYPES[kind]).min, _gen(classes)
+    x = torch.randn(16, classes, device="cuda", generator=g) * 4
+    x[1] = -math.inf
+    x[2, 1:] = -math.inf
+    x[3] = low
+    x[4, ::2] = low
+    x[5, 2] = math.nan
+    x[6, 3] = math.inf
+    x[7] = torch.arange(classes, device="cuda") % 5
+    x[8, ::3] = -math.inf
+    x[9] = torch.arange(classes, device="cuda").float() / 50          # (in bfloat16: many equal ones)
+    x[10] = -x[9]
+    x[11] = 2.5
+    x[12, :: max(classes // 9, 1)] = 9.0
+    x[13, 1], x[13, 4] = math.nan, math.nan
+    x[14, ::64] = torch.arange(-(-classes // 64), device="cuda") + 20.0   # all of the best in one lane's share
+    x = x.to(TYPES[kind])
+    tokens = torch.stack([torch.arange(16, device="cuda") % classes, torch.full((16,), classes - 1, device="cuda")], 1)
+    for top in sorted({0, 1, 3, min(9, classes), min(64, classes)} & set(range(classes + 1))):
+        got = ops.token_logprobs(x.repeat(260, 1), tokens.repeat(260, 1), top=top)
+        _check_scores(x, tokens, top, [t[:16] for t in got])
+        for t in got:
+            block = t.view(260, 16, -1)
+            assert torch.equal(block.view(torch.int32), block[:1].expand_as(block).contiguous().view(torch.int32))
+
+
+@pytest.mark.gpu
+def test_gpu_logprobs_millions_of_rows():
+    """more rows than the first axis of a grid holds: the last ones answer as they do alone"""
+    rows, classes = (1 << 21) + 3000, 270
+    x = torch.randn(3000, classes, device="cuda", generator=_gen(21)).bfloat16()
+    many = torch.zeros(rows, classes, device="cuda", dtype=torch.bfloat16)
+    many[-3000:] = x
+    tokens = torch.randint(0, classes, (3000,), device="cuda", generator=_gen(22))
+    all_tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    all_tokens[-3000:] = tokens
+    for a, b in zip(ops.token_logprobs(many, all_tokens, top=9), ops.token_logprobs(x, tokens, top=9)):
+        assert torch.equal(a[-3000:], b)
+
+
+@pytest.mark.gpu
 def test_gpu_python_refusals():
     pages = ops.kv_pages(4, 2, 16, 64)
     k, v, slots = torch.zeros(3, 2, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda"), torch.arange(3, device="cuda")
