@@ -394,7 +394,7 @@ typedef struct pocr_kv_pages {
 } pocr_kv_pages;
 /* Keys and values to be written: k, v [tokens][kv_heads][head_dim] of `dtype` with element strides per token and head (the last axis is
  * contiguous) -> the rows of slots[tokens] (int64 when slots64, else int32).  A slot outside the cache (-1: padding) is skipped.  Slots of
- * one call are distinct: a slot named twice holds a mixture of the rows given for it. */
+ * one call are distinct: a slot named twice holds a mixture of the rows given for it.  2 * tokens * kv_heads * head_dim is at most 2^34 (so for reads). */
 typedef struct pocr_kv_rows {
     const void *k, *v, *slots;
     int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride, tokens;
@@ -412,8 +412,8 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const 
  * A row whose mask leaves nothing gets out = 0 and lse = -inf.  Query head h reads key head h / (heads / kv_heads).
  * A position beyond the page table or whose page id is outside the cache is absent: nobody sees it and it is never read.
  * q_start is non-decreasing from 0 and ends at or below `tokens`; rows of out / lse behind q_start[seqs] are left as they were, or zeroed
- * (lse: -inf) with zero_rest.  max_queries: the most new tokens of one sequence, if known (0: unknown): it shapes the launch, any
- * value gives the same answer.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
+ * (lse: -inf) with zero_rest.  max_queries: the most new tokens of one sequence, if known (0: unknown): it shapes the launch; any
+ * value gives the same answer but for the order of the sums.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
 typedef struct pocr_tree_attention_args {
     const void *q;                    /* [tokens][heads][head_dim], element strides q_token_stride, q_head_stride; rows start at multiples of 16 bytes */
     void *out;                        /* [tokens][heads][head_dim] contiguous, 16-byte aligned */
@@ -434,7 +434,7 @@ int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *pages,
  *   entropy [rows]          : -sum p log p
  *   top_logprob, top_index [rows][top] : the `top` largest logits, 0 <= top <= min(64, classes), equal ones in the order of their index, NaN first
  * A logit of -inf has probability 0; a row of nothing else has log probabilities -inf and entropy 0; a row with NaN or +inf has NaN.
- * Sums are in 32 bits. */
+ * Rows: fewer than 2^28 to 512 classes, 2^26 to 4096, 2^24 to 32768, 2^22 above.  Sums are in 32 bits. */
 typedef struct pocr_token_logprobs_args {
     const void *logits, *tokens;
     float *logprob, *entropy, *top_logprob;

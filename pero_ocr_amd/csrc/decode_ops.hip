@@ -117,21 +117,23 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     const int64_t average = (t->tokens + t->seqs - 1) / t->seqs, group = t->heads / c->kv_heads, known = std::min(t->max_queries, t->tokens);
     p.rt = (known > 0 ? known : average) * group > 16 && two_tiles(t->dtype, c->head_dim) ? 2 : 1;
     // Slots for row tiles: the same number for each sequence where that is not more than what their rows could need together (then nothing has to
-    // be looked up: 2048 sequences of 8 tokens 510 us, looked up 615 us), or as many as its rows need (8 single tokens next to one of
+    // be looked up: 2048 sequences of 8 tokens 510 us, looked up 615 us), or as many as its rows need (15 single tokens next to one of
     // 512: 81 us, slots for 512 in each 114 us; 256 single tokens of which nobody said so 53 us, slots for all of them in each 295 us).
     const int64_t all = t->tokens * group / (16 * p.rt), most = known > 0 ? (known * group + 16 * p.rt - 1) / (16 * p.rt) : all + 1;
     p.tiles = most * t->seqs <= all + t->seqs ? (int)most : 0;
     p.slots = p.tiles ? p.tiles * (int64_t)t->seqs : all + t->seqs;
     const int64_t units = (p.tiles ? p.slots : all + (t->seqs + 1) / 2) * c->kv_heads, blocks = (((int64_t)t->max_pages << page_shift(c)) + 31) / 32;
     // Splits for one workgroup on each CU, of 10 blocks of 32 keys or more: a workgroup costs about 4 us to start and to end (single tokens, 8 key
-    // heads of 128, 4 query heads each; in brackets the rule's: 500 keys [1] 8.6 us, 2 splits 10.0; 2000 keys 1 split 17.3, 3 12.9, [6] 11.4;
+    // heads of 128, 8 query heads each; in brackets the rule's: 500 keys [1] 8.6 us, 2 splits 10.0; 2000 keys 1 split 17.3, 3 12.9, [6] 11.4;
     // 8 sequences of 4000 keys 1 split 29.8, 2 21.8, [4] 19.0, 6 20.6; 32 sequences [1] 47, 2 49).  Two workgroups on each where a split still is
     // 256 blocks, so that sequences of different lengths end together (60 to 131 thousand keys: 256 workgroups 186 us, 512 169 us, 768 172 us).
     p.nsplit = (int)std::min<int64_t>({std::max({std::min(256 / units, blocks / 10), std::min(512 / units, blocks / 256), (int64_t)1}), TA_MAX_SPLITS,
                                        std::max<int64_t>((1 << 26) / (t->tokens * t->heads), 1)});
+    // A wave alone where there are enough of them for 8 on a CU: nothing to join (512 single tokens over 40 to 272 keys 25.2 us, four waves 33.8;
+    // 256 over 2000 keys 183 and 195).
     p.waves = p.rt == 1 && units >= 2048 ? 1 : 4;
-    // Lists of slots: one for every key head and split.  Tiles of a sequence share their XCD's L2 when a list stays on one XCD (24 trees, 128 rows:
-    // 204 us, in runs of 8 slots 227, of 2 292, of 1 375); with lists that 8 XCDs cannot share evenly, in runs of up to 16.
+    // Lists of slots: one for every key head and split.  Tiles of a sequence share their XCD's L2 when a list stays on one XCD (24 trees of 28 to 256
+    // rows: 204 us, in runs of 8 slots 227, of 2 292, of 1 375); with lists that 8 XCDs cannot share evenly, in runs of up to 16.
     const int64_t lists = (int64_t)c->kv_heads * p.nsplit, work = p.slots * lists;
     p.run = 1;
     if (p.tiles != 1) {
