@@ -118,7 +118,7 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     p.rt = (known > 0 ? known : average) * group > 16 && two_tiles(t->dtype, c->head_dim) ? 2 : 1;
     // Slots for row tiles: the same number for each sequence where that is not more than what their rows could need together (then nothing has to
     // be looked up: 2048 sequences of 8 tokens 510 us, looked up 615 us), or as many as its rows need (15 single tokens next to one of
-    // 512: 81 us, slots for 512 in each 114 us; 256 single tokens of which nobody said so 53 us, slots for all of them in each 295 us).
+    // 512: 82 us, slots for 512 in each 114 us; 256 single tokens of which nobody said so 53 us, slots for all of them in each 295 us).
     const int64_t all = t->tokens * group / (16 * p.rt), most = known > 0 ? (known * group + 16 * p.rt - 1) / (16 * p.rt) : all + 1;
     p.tiles = most * t->seqs <= all + t->seqs ? (int)most : 0;
     p.slots = p.tiles ? p.tiles * (int64_t)t->seqs : all + t->seqs;
@@ -132,15 +132,12 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     // A wave alone where there are enough of them for 8 on a CU: nothing to join (512 single tokens over 40 to 272 keys 25.2 us, four waves 33.8;
     // 256 over 2000 keys 183 and 195).
     p.waves = p.rt == 1 && units >= 2048 ? 1 : 4;
-    // Lists of slots: one for every key head and split.  Tiles of a sequence share their XCD's L2 when a list stays on one XCD (24 trees of 28 to 256
-    // rows: 204 us, in runs of 8 slots 227, of 2 292, of 1 375); with lists that 8 XCDs cannot share evenly, in runs of up to 16.
+    // Lists of slots, one for every key head and split: each on one XCD where 8 XCDs share them evenly (24 trees of 28 to 256 rows: 202 us, in runs of 8
+    // slots 227, of 2 292, of 1 375), in runs of up to 16 where not.
     const int64_t lists = (int64_t)c->kv_heads * p.nsplit, work = p.slots * lists;
-    p.run = 1;
-    if (p.tiles != 1) {
-        if (lists % 8 == 0) p.run = p.slots;
-        else while (p.run < 16 && work / p.run >= 128) p.run *= 2;
-    }
-    p.groups = (work + 8 * p.run - 1) / (8 * p.run) * (8 * p.run);
+    p.run = p.tiles == 1 || lists % 8 ? 1 : 0;
+    while (p.tiles != 1 && p.run > 0 && p.run < 16 && work / p.run >= 128) p.run *= 2;
+    p.groups = p.run ? (work + 8 * p.run - 1) / (8 * p.run) * (8 * p.run) : work;
     return p;
 }
 

@@ -288,20 +288,47 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
             for (int64_t p = (int64_t)blockIdx.x * (64 * NW) + tid; p < rest; p += all) a.lse[from + p] = -INFINITY;
     }
 
-    // Consecutive workgroups go to different XCDs; runs of `run` slots stay on one, so that the row tiles of one sequence and key head, which
-    // read the same keys, share an L2.  With one tile a sequence, key heads are next to each other instead: no XCD has a long sequence to itself.
-    const uint32_t turn = (blockIdx.x >> 3) / a.run, number = (turn * 8 + (blockIdx.x & 7)) * a.run + ((blockIdx.x >> 3) - turn * a.run);
-    const uint32_t group = (uint32_t)a.heads / (uint32_t)a.kv_heads, pairs = a.slots * (uint32_t)a.kv_heads;
-    const int split = (int)(number / pairs);
-    const uint32_t pair = number - (uint32_t)split * pairs, slot = a.tiles == 1 ? pair / (uint32_t)a.kv_heads : pair % a.slots;
-    const int hk = (int)(a.tiles == 1 ? pair - slot * (uint32_t)a.kv_heads : pair / a.slots);
+    // A list of slots for each key head and split.  Row tiles of one sequence and key head read the same keys, so they should share an L2, and consecutive
+    // workgroups go to different XCDs: every list stays on one XCD (run = 0; the XCD's lists side by side, so that unused slots come
+    // last), or runs of `run` slots do.  With one tile a sequence, key heads are next to each other instead: no XCD has a long sequence to itself.
+    const uint32_t kv_heads = (uint32_t)a.kv_heads, group = (uint32_t)a.heads / kv_heads, rest8 = blockIdx.x >> 3, xcd = blockIdx.x & 7;
+    uint32_t list, slot;
+    if (a.run == 0) {
+        const uint32_t own = kv_heads * (uint32_t)a.nsplit / 8;       // lists of an XCD
+        slot = rest8 / own;
+        list = (rest8 - slot * own) * 8 + xcd;
+    } else {
+        const uint32_t turn = rest8 / a.run, number = (turn * 8 + xcd) * a.run + (rest8 - turn * a.run);
+        if (a.tiles == 1) {
+            const uint32_t at = number / kv_heads, split0 = at / a.slots;
+            slot = at - split0 * a.slots;
+            list = split0 * kv_heads + (number - at * kv_heads);
+        } else {
+            list = number / a.slots;
+            slot = number - list * a.slots;
+        }
+    }
+    const int split = (int)(list / kv_heads), hk = (int)(list - (uint32_t)split * kv_heads);
     if (split >= a.nsplit) return;
-    // Slots: `tiles` for each sequence, or (tiles = 0) as many as its rows need: sequence s then begins at slot_of(first row), which leaves it
-    // one more than its whole tiles.
+    // Slots: `tiles` for each sequence, or (tiles = 0) as many as its rows need, counted where a wave has a lane for each sequence; where not, sequence
+    // s begins at slot_of(first row), which leaves it one more than its whole tiles.
     auto slot_of = [&](int32_t first, int i) { return (uint32_t)min(max(first, 0), (int32_t)a.tokens) * group / (16 * RT) + (uint32_t)i; };
     int s = 0;
+    uint32_t first_slot = 0;
     if (a.tiles) s = (int)(slot / (uint32_t)a.tiles);
-    else {
+    else if (a.seqs <= 64) {
+        const int32_t total = (int32_t)a.tokens, b = min(max(a.starts[min(lane, a.seqs - 1)], 0), total), e = min(a.starts[min(lane, a.seqs - 1) + 1], total);
+        const int own = lane < a.seqs ? (int)(((uint32_t)max(e - b, 0) * group + 16 * RT - 1) / (16 * RT)) : 0;
+        int until = own;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int before = __shfl_up(until, o, 64);
+            until += lane >= o ? before : 0;
+        }
+        s = (int)__popcll(__ballot(until <= (int)slot));
+        if (s >= a.seqs) return;
+        first_slot = (uint32_t)__builtin_amdgcn_readlane(until - own, s);
+    } else {
         int left = a.seqs;
         while (left > 1) {                                            // the last sequence that begins at or before this slot: 64 looked at in a step
             const int step = (left + 63) / 64, at = s + min(lane * step, left - 1);
@@ -312,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
         s = __builtin_amdgcn_readfirstlane(s);
     }
     const TreeSeq sq = tree_seq(a, s);
-    const uint32_t rows = (uint32_t)sq.n * group, tile0 = slot - (a.tiles ? (uint32_t)(s * a.tiles) : slot_of(sq.first, s));
+    const uint32_t rows = (uint32_t)sq.n * group, tile0 = slot - (a.tiles ? (uint32_t)(s * a.tiles) : a.seqs <= 64 ? first_slot : slot_of(sq.first, s));
     if (tile0 >= (rows + 16 * RT - 1) / (16 * RT)) return;            // an unused slot, or a sequence without new tokens
     const int32_t *table = a.table + s * a.table_stride;
     // scores in units of log2: the sign of the scale goes to the query, so that the largest product is the largest score; 0 makes the query 0
