@@ -190,10 +190,12 @@ int check_scores(const pocr_token_logprobs_args *t) {
 }
 
 // Workgroups of a row: more than one where rows are too few to fill the chip and so long that one workgroup (36 GB/s) takes longer than
-// the second launch and the join (9 rows of 604 KB: whole 16.5 us, in slices 17.0 us).
+// the second launch and the join (9 rows of 151003 in fp32, top 8: whole 16.0 us, in slices 11.6; 64 of 152000 in bf16 16.1 and 12.9; 8 of 80000,
+// top 5, 11.5 and 10.6, top 64 13.7 and 15.7; 100 of 152000 19.5 and 19.2), up to four on each CU (64 rows of 400000 in fp32: 256 workgroups 41 us,
+// 512 28.3, 1024 27.4, whole 39), of 8192 classes or more.
 int score_slices(const pocr_token_logprobs_args *t) {
-    if ((int64_t)t->classes * elem_size(t->dtype) <= 786432 || t->rows >= 128) return 1;
-    return (int)std::min<int64_t>({(256 + t->rows - 1) / t->rows, t->classes / 8192, 64, LP_CAND / std::max(t->top, 1)});
+    if (t->classes <= 98304 || t->rows >= 128) return 1;
+    return (int)std::min<int64_t>({(1024 + t->rows - 1) / t->rows, t->classes / 8192, 64, LP_CAND / std::max(t->top, 1)});
 }
 
 int64_t score_workspace(const pocr_token_logprobs_args *t) {

@@ -168,8 +168,8 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
 // the list of candidates, and rows with NaN or +inf, take one pass per alternative.
 // Few long rows are cut into slices, a workgroup each (SPLIT), whose sums and alternatives the kernel below joins.
 //
-// Bound by HBM where rows are long (1024 rows of 131072 in bf16, top 20: 52.7 us = 5.1 TB/s; 9 rows of 151003 in fp32, which 9 CUs read: 16.5 us, 36
-// GB/s a CU); where they are short by the choice of the alternatives, which a wave makes alone (36864 rows of 1000 in fp32: none 30.5 us, top 4 47.5,
+// Bound by HBM where rows are long (1024 rows of 131072 in bf16, top 20: 52.7 us = 5.1 TB/s; 9 rows of 151003 in fp32 in 18 slices each 11.6 us,
+// read by 9 CUs 16.0, 36 GB/s a CU); where they are short by the choice of the alternatives, which a wave makes alone (36864 rows of 1000 in fp32: none 30.5 us, top 4 47.5,
 // top 20 64).  So reductions stay in registers, and the list of a single wave is short: 2.6 KB of LDS let 32 of them share a CU (with 9 KB 17,
 // 52 -> 33 us for rows of 500, top 4).
 constexpr int LP_CAND = 1024, LP_SLACK = 32, LP_GRID = 1 << 21;       // (rows in the first axis of the grid)
@@ -371,17 +371,30 @@ __global__ __launch_bounds__(B) void token_logprobs_kernel(LogprobArgs a) {
     }
 }
 
-// The slices of a row meet: a workgroup per row; a lane per slice for the sums, the alternatives ranked among all slices'.
+// The slices of a row meet: a workgroup per row; a lane per slice for the sums.  Every slice's alternatives come in order, so a row's k best reach
+// the least of the slices' ceil(k / slices)-th ones (these and the better ones are k or more), and the best of the slices' k-th ones; only what
+// does is ranked (16 slices, k = 64: all 1024 against each other took 60 us).
 template <int DT>
 __global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogprobArgs a) {
-    __shared__ unsigned long long cand[LP_CAND];
+    __shared__ unsigned long long cand[LP_CAND], limit;
     __shared__ float whole[2];
+    __shared__ int kept;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const int n = a.slices * a.top;                             // <= LP_CAND
     const unsigned long long *found = reinterpret_cast<const unsigned long long *>(a.part + a.rows * a.slices * 4) + r * n;
-    for (int i = tid; i < n; i += 256) cand[i] = found[i];
-    if (tid < 64) {                                             // (slices <= 64)
+    if (tid < 64 && a.top > 0) {                                // (slices <= 64)
+        const int at = min(tid, a.slices - 1) * a.top;
+        unsigned long long least = found[at + (a.top + a.slices - 1) / a.slices - 1], last = found[at + a.top - 1];
+        for (int o = 32; o >= 1; o >>= 1) {
+            const unsigned long long p = __shfl_xor(least, o, 64), q = __shfl_xor(last, o, 64);
+            least = p < least ? p : least;
+            last = q > last ? q : last;
+        }
+        if (tid == 0) limit = least > last ? least : last;
+    }
+    if (tid == 64) kept = 0;
+    if (tid < 64) {
         float4 s = make_float4(-INFINITY, 0.f, 0.f, 0.f);
         if (tid < a.slices) s = *reinterpret_cast<const float4 *>(a.part + (r * a.slices + tid) * 4);
         float m = s.x, z = s.y, e = s.z;
@@ -402,10 +415,17 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogprobArgs a)
     const float m = whole[0], base = m == -INFINITY ? 0.f : m, logz = whole[1];
     const bool none = logz == -INFINITY;
     lp_given(a, r, tid, 256, base, logz, none);
+    if (a.top == 0) return;
     for (int i = tid; i < n; i += 256) {
+        const unsigned long long c = found[i];
+        if (c >= limit) cand[atomicAdd(&kept, 1)] = c;
+    }
+    __syncthreads();
+    const int left = kept;
+    for (int i = tid; i < left; i += 256) {
         const unsigned long long c = cand[i];
         int rank = 0;
-        for (int q = 0; q < n; ++q) rank += cand[q] > c;
+        for (int q = 0; q < left; ++q) rank += cand[q] > c;
         if (rank < a.top) {
             a.top_logprob[r * a.top + rank] = none ? -INFINITY : (lp_value((uint32_t)(c >> 32)) - base) - logz;
             a.top_index[r * a.top + rank] = (int32_t)~(uint32_t)c;
