@@ -279,11 +279,12 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
     __shared__ float stat[NW][RT * 16][2], whole[RT * 16][2];
     __shared__ int64_t place_of[RT * 16];
 
-    if (a.zero_rest) {                                                // rows of no sequence, a share for every workgroup
+    if (a.zero_rest) {                                                // rows of no sequence, a share for every workgroup; 1: out and lse, 2: lse alone
         const int32_t end = min(max(((ScalarInts)a.starts)[a.seqs], 0), (int32_t)a.tokens);
         const int64_t from = (int64_t)end * a.heads, rest = (a.tokens - end) * a.heads, all = (int64_t)gridDim.x * (64 * NW);
         constexpr int PIECES = D * sizeof(T) / 16;
-        for (int64_t p = (int64_t)blockIdx.x * (64 * NW) + tid; p < rest * PIECES; p += all) static_cast<kv_u32x4 *>(a.out)[from * PIECES + p] = (kv_u32x4){0, 0, 0, 0};
+        if (a.zero_rest != 2)
+            for (int64_t p = (int64_t)blockIdx.x * (64 * NW) + tid; p < rest * PIECES; p += all) static_cast<kv_u32x4 *>(a.out)[from * PIECES + p] = (kv_u32x4){0, 0, 0, 0};
         if (a.lse)
             for (int64_t p = (int64_t)blockIdx.x * (64 * NW) + tid; p < rest; p += all) a.lse[from + p] = -INFINITY;
     }

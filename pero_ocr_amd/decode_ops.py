@@ -210,8 +210,8 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
     lies outside the cache (-1) are absent.  scale: head_dim ** -0.5 unless given.  max_queries: the most new tokens of one sequence,
     if the caller knows it (it shapes the launch; the answer differs at most by the order of its sums).
 
-    -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros
-    (lse -inf) in a tensor made here and are left alone in an `out` of the caller's (contiguous)."""
+    -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros in a
+    tensor made here and are left alone in an `out` of the caller's (contiguous); lse, always made here, has -inf there."""
     n, index = pages.native, pages.index
     if not (type(q) is _Tensor and type(page_table) is _Tensor and type(lengths) is _Tensor and type(q_start) is _Tensor and q.dtype in _DTYPES
             and page_table.dtype is _INT and lengths.dtype is _INT and q_start.dtype is _INT and q.dim() == 3 and page_table.dim() == 2
@@ -253,7 +253,7 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
         args = _native.TreeAttentionArgs(
             at, out.data_ptr(), lse.data_ptr() if want_lse else None, page_table.data_ptr(), lengths.data_ptr(), q_start.data_ptr(),
             mask.data_ptr() if mask is not None else None, None, 0, qs[0], qs[1], ps[0], mask.stride(0) if mask is not None else 0, tokens, int(max_queries),
-            _DTYPES[q.dtype], seqs, heads, width, mask.shape[1] if mask is not None else 0, fresh, dim ** -0.5 if scale is None else float(scale))
+            _DTYPES[q.dtype], seqs, heads, width, mask.shape[1] if mask is not None else 0, 1 if fresh else 2 if want_lse else 0, dim ** -0.5 if scale is None else float(scale))
         need = lib.pocr_tree_attention_workspace(n, args)
         if need:
             if need < 0:
