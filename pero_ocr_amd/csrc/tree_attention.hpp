@@ -25,8 +25,9 @@
 // tokens over 40 to 272 keys of 64, fp32, 25 us, where a wave has 2 to 6 blocks and the start and the end of a workgroup (4 us) weigh most.
 //
 // A NaN or infinity in V spreads in a matrix product to the masked rows, whose probability is 0; testing every element for it costs more than the
-// transposition, so the loop does not.  A wave whose sums come out not finite goes through its keys again one by one, every row with the
-// keys that it sees: slow, and met only where such numbers are.
+// transposition, so the loop does not.  Finite values near the end of the range may pass it in a sum of up to 2^8 times each, where the
+// average does not.  A wave whose sums come out not finite goes through its keys again one by one, every row with the keys that it sees, and sums
+// the average itself: slow, and met only where such numbers are.  Waves and splits meet as averages, weighted with their share of the row's sum.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -47,7 +48,7 @@ struct TreeAttnArgs {
     const uint64_t *mask;
     void *out;
     float *lse;
-    float *part;                  // nsplit > 1: sums [nsplit][tokens * heads][D], then (maximum, sum) [nsplit][tokens * heads][2]
+    float *part;                  // nsplit > 1: averages [nsplit][tokens * heads][D], then (maximum, sum) [nsplit][tokens * heads][2]
     int64_t q_ts, q_hs, table_stride, mask_stride, tokens;
     int32_t seqs, heads, kv_heads, num_pages, page_shift, max_pages, mask_words, zero_rest, nsplit, tiles;
     uint32_t slots, run;
@@ -518,36 +519,44 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
             for (int t = 0; t < NB; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) odd = fmaf(o[rt][t][r], 0.f, odd);
-        if (__ballot(odd != odd)) {                                          // key by key, each row only with what it sees
+        float share[RT];                                              // what o is to be weighted with: 1, or the wave's sum where o is an average already
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) share[rt] = 1.f;
+        if (__ballot(odd != odd)) {                                          // key by key, each row only with what it sees: its sum first, then the average
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 m[rt] = -INFINITY;
-                l[rt] = 0.f;
+                share[rt] = 0.f;
 #pragma unroll
                 for (int t = 0; t < NB; ++t) o[rt][t] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
                 const uint32_t rr = min(r0 + 16 * rt + row, rows - 1);
                 const T *qr = static_cast<const T *>(a.q) + (int64_t)(sq.first + tok[rt]) * a.q_ts + (hk * (int)group + (int)(rr - (uint32_t)tok[rt] * group)) * a.q_hs;
-                for (int32_t b = first_block + wave; b < end_block; b += NW)
-                    for (int32_t key = b << 5, n = min(32, sq.len - key); n > 0; --n, ++key) {
-                        const int64_t kr = kv_row_base(table, a.max_pages, a.num_pages, a.kv_heads, hk, a.page_shift, key);
-                        if (kr < 0) continue;                         // (the same for all lanes)
-                        float dot = 0.f;
 #pragma unroll 1
-                        for (int d = g * (D / 4); d < (g + 1) * (D / 4); ++d) dot += (float)qr[d] * csign * kv_element<FMT>(a.k, a.k_exp, kr, D, d);
-                        dot = row_sum(dot);
-                        const bool sees = tree_window(a.mask ? a.mask + (int64_t)(sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], key - ctx) & 1;
-                        if (!sees) continue;
-                        const float mx = fmaxf(m[rt], dot);
-                        const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[rt] - mx) * cabs);
-                        const float mc = mx == -INFINITY ? 0.f : mx * cabs, p = __builtin_amdgcn_exp2f(fmaf(dot, cabs, -mc));
-                        m[rt] = mx;
-                        l[rt] = l[rt] * alpha + (g == 0 ? p : 0.f);
+                for (int turn = 0; turn < 2; ++turn) {
+                    const float inv = share[rt] == 0.f ? 0.f : 1.f / share[rt];
+                    for (int32_t b = first_block + wave; b < end_block; b += NW)
+                        for (int32_t key = b << 5, n = min(32, sq.len - key); n > 0; --n, ++key) {
+                            const int64_t kr = kv_row_base(table, a.max_pages, a.num_pages, a.kv_heads, hk, a.page_shift, key);
+                            if (kr < 0) continue;                     // (the same for all lanes)
+                            float dot = 0.f;
+#pragma unroll 1
+                            for (int d = g * (D / 4); d < (g + 1) * (D / 4); ++d) dot += (float)qr[d] * csign * kv_element<FMT>(a.k, a.k_exp, kr, D, d);
+                            dot = row_sum(dot);
+                            const bool sees = tree_window(a.mask ? a.mask + (int64_t)(sq.first + tok[rt]) * a.mask_stride : nullptr, a.mask_words, tok[rt], key - ctx) & 1;
+                            if (!sees) continue;
+                            const float mx = fmaxf(m[rt], dot), mc = mx == -INFINITY ? 0.f : mx * cabs, p = __builtin_amdgcn_exp2f(fmaf(dot, cabs, -mc));
+                            if (turn == 0) {
+                                share[rt] = share[rt] * (m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[rt] - mx) * cabs)) + p;
+                                m[rt] = mx;
+                            } else {
 #pragma unroll
-                        for (int t = 0; t < NB; ++t)
+                                for (int t = 0; t < NB; ++t)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                o[rt][t][e] = (alpha == 1.f ? o[rt][t][e] : o[rt][t][e] * alpha) + p * kv_element<FMT>(a.v, a.v_exp, kr, D, g * (D / 4) + e * NB + t);
-                    }
+                                    for (int e = 0; e < 4; ++e) o[rt][t][e] += p * inv * kv_element<FMT>(a.v, a.v_exp, kr, D, g * (D / 4) + e * NB + t);
+                            }
+                        }
+                }
+                l[rt] = g == 0 ? share[rt] : 0.f;
             }
         }
 #pragma unroll
@@ -573,7 +582,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 const float mw = stat[w][16 * rt + row][0];
                 ll += stat[w][16 * rt + row][1] * (mw == mm || mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mw - mm) * cabs));      // (no maximum: 0 or NaN)
             }
-            const float f = m[rt] == mm || m[rt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[rt] - mm) * cabs);
+            // (averages: of finite values they are finite, however many there are)
+            const float f = (m[rt] == mm || m[rt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[rt] - mm) * cabs)) * share[rt] * (ll == 0.f ? 0.f : 1.f / ll);
             float *dst = &osum[wave][16 * rt + row][g * (D / 4)];
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -602,10 +612,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                     ml[1] = ll;
                 }
             } else {
-                const float inv = ll == 0.f ? 0.f : 1.f / ll;
                 alignas(16) T x[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = (T)(ll == 0.f ? 0.f : v[j] * inv);
+                for (int j = 0; j < 4; ++j) x[j] = (T)(ll == 0.f ? 0.f : v[j]);
                 T *po = static_cast<T *>(a.out) + to * D + d;
                 if constexpr (sizeof(T) == 4) *reinterpret_cast<kv_u32x4 *>(po) = *reinterpret_cast<const kv_u32x4 *>(x);
                 else *reinterpret_cast<kv_u32x2 *>(po) = *reinterpret_cast<const kv_u32x2 *>(x);
@@ -616,7 +625,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
     }
 }
 
-// The splits' sums of one row meet: a wave per (token, head) of a sequence.  Rows of no sequence are left to the kernel above.  A chain of three round
+// The splits' averages of one row meet: a wave per (token, head) of a sequence.  Rows of no sequence are left to the kernel above.  A chain of three round
 // trips to memory: 4 us for 1056 rows of 6 splits.
 constexpr int TA_MAX_SPLITS = 128;
 
@@ -647,6 +656,8 @@ __global__ __launch_bounds__(256) void tree_attention_join_kernel(TreeAttnArgs a
         l += f[i] * ls[i];
     }
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) f[i] = l == 0.f ? 0.f : f[i] * ls[i] / l;          // a split's share of the row
     const float *po = a.part + (int64_t)at * D + (D < 64 ? lane & (D - 1) : lane * E);
     auto add = [&](auto width) {                                      // sums on their way at once: a launch of few rows is a chain of round trips
         constexpr int U = decltype(width)::value;
@@ -670,7 +681,7 @@ __global__ __launch_bounds__(256) void tree_attention_join_kernel(TreeAttnArgs a
     T *out = static_cast<T *>(a.out) + (int64_t)at * D + lane * E;
     if (lane * E < D) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) out[e] = (T)(l == 0.f ? 0.f : acc[e] / l);
+        for (int e = 0; e < E; ++e) out[e] = (T)(l == 0.f ? 0.f : acc[e]);
     }
     if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147180559945f;
 }
