@@ -412,8 +412,9 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const 
  * A row whose mask leaves nothing gets out = 0 and lse = -inf.  Query head h reads key head h / (heads / kv_heads).
  * A position beyond the page table or whose page id is outside the cache is absent: nobody sees it and it is never read.
  * q_start is non-decreasing from 0 and ends at or below `tokens`; rows of out / lse behind q_start[seqs] are left as they were (zero_rest 0),
- * or become 0 and -inf (1), or -inf in lse while out is left alone (2).  max_queries: the most new tokens of one sequence, if known (0: unknown): it shapes the launch; any
- * value gives the same answer but for the order of the sums.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
+ * or become 0 and -inf (1), or -inf in lse while out is left alone (2).  max_queries: the most new tokens of
+ * one sequence, if known (0: unknown): it shapes the launch and the workspace (at most 17 MB); any value gives the same answer but for the order of the
+ * sums, one below the truth later.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
 typedef struct pocr_tree_attention_args {
     const void *q;                    /* [tokens][heads][head_dim], element strides q_token_stride, q_head_stride; rows start at multiples of 16 bytes */
     void *out;                        /* [tokens][heads][head_dim] contiguous, 16-byte aligned */

@@ -110,7 +110,7 @@ template <int E> dim3 row_grid(uint32_t rows, int D) { const uint32_t per = 256 
 constexpr bool two_tiles(int dtype, int D) { return D <= 64 || (D == 128 && dtype != POCR_F32); }
 
 // How the work of one attention call is cut.
-struct AttendPlan { int rt, tiles, nsplit, waves; int64_t slots, run, groups; };
+struct AttendPlan { int rt, tiles, nsplit, waves; int64_t slots, run, groups, part_rows, tile_rows; };
 
 AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
     AttendPlan p;
@@ -127,8 +127,14 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     // heads of 128, 8 query heads each; in brackets the rule's: 500 keys [1] 8.6 us, 2 splits 10.0; 2000 keys 1 split 17.3, 3 12.9, [6] 11.4;
     // 8 sequences of 4000 keys 1 split 29.8, 2 21.8, [4] 19.0, 6 20.6; 32 sequences [1] 47, 2 49).  Two workgroups on each where a split still is
     // 256 blocks, so that sequences of different lengths end together (60 to 131 thousand keys: 256 workgroups 186 us, 512 169 us, 768 172 us).
-    p.nsplit = (int)std::min<int64_t>({std::max({std::min(256 / units, blocks / 10), std::min(512 / units, blocks / 256), (int64_t)1}), TA_MAX_SPLITS,
-                                       std::max<int64_t>((1 << 26) / (t->tokens * t->heads), 1)});
+    p.nsplit = (int)std::min<int64_t>(std::max({std::min(256 / units, blocks / 10), std::min(512 / units, blocks / 256), (int64_t)1}), TA_MAX_SPLITS);
+    // Room for the splits of the rows that the slots hold (units * nsplit <= 512: at most 17 MB), not of all that a batch is padded to.
+    p.tile_rows = p.tiles * (int64_t)(16 * p.rt);
+    p.part_rows = p.tile_rows * t->seqs * c->kv_heads;
+    if (p.tiles == 0 || p.part_rows >= t->tokens * t->heads) {
+        p.tile_rows = 0;
+        p.part_rows = t->tokens * t->heads;
+    }
     // A wave alone where there are enough of them for 8 on a CU: nothing to join (512 single tokens over 40 to 272 keys 25.2 us, four waves 33.8;
     // 256 over 2000 keys 183 and 195).
     p.waves = p.rt == 1 && units >= 2048 ? 1 : 4;
@@ -141,6 +147,8 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     return p;
 }
 
+int64_t attend_workspace(const pocr_kv_pages *c, const AttendPlan &p) { return p.nsplit == 1 ? 0 : p.nsplit * p.part_rows * (c->head_dim + 2) * 4; }
+
 template <int DT, int FMT, int D> int attend(const AttendPlan &p, void *stream, const TreeAttnArgs &a) {
     const char *w = "pocr_tree_attention";
     const dim3 grid((unsigned)p.groups), block(64 * p.waves);
@@ -149,7 +157,7 @@ template <int DT, int FMT, int D> int attend(const AttendPlan &p, void *stream, 
                    : p.rt == 1  ? launch(w, tree_attention_kernel<DT, FMT, D, 1, 4>, grid, block, stream, a)
                                 : launch(w, tree_attention_kernel<DT, FMT, D, RT, 4>, grid, block, stream, a);
     if (rc || p.nsplit == 1) return rc;
-    return launch(w, tree_attention_join_kernel<DT, D>, dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), stream, a);
+    return launch(w, tree_attention_join_kernel<DT, D>, p.tile_rows ? dim3(a.tile_rows / 4, a.kv_heads, a.seqs) : dim3((unsigned)((p.part_rows + 3) / 4)), dim3(256), stream, a);
 }
 
 template <int DT, int FMT> int attend_by_dim(int D, const AttendPlan &p, void *stream, const TreeAttnArgs &a) {
@@ -279,8 +287,7 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *c, const void
 int64_t pocr_tree_attention_workspace(const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
     if (check_attention(c, t)) return -1;
     if (t->tokens == 0) return 0;
-    const AttendPlan p = attend_plan(c, t);
-    return p.nsplit == 1 ? 0 : (int64_t)p.nsplit * t->tokens * t->heads * (c->head_dim + 2) * 4;
+    return attend_workspace(c, attend_plan(c, t));
 }
 
 int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, const pocr_tree_attention_args *t) {
@@ -293,14 +300,15 @@ int pocr_tree_attention(int device_id, void *stream, const pocr_kv_pages *c, con
     if (!aligned(t->out, 16) || !aligned(t->lse, 4) || !aligned(t->mask, 8) || !aligned(t->lengths, 4) || !aligned(t->q_start, 4) || !aligned(t->page_table, 4))
         return refuse("pocr_tree_attention: a pointer is not aligned to its element (out: to 16 bytes)");
     const AttendPlan p = attend_plan(c, t);
-    const int64_t need = p.nsplit == 1 ? 0 : (int64_t)p.nsplit * t->tokens * t->heads * (c->head_dim + 2) * 4;
+    const int64_t need = attend_workspace(c, p);
     if (need > 0 && (!t->workspace || !aligned(t->workspace, 16) || t->workspace_bytes < need))
         return refuse("pocr_tree_attention: a workspace of %lld bytes, aligned to 16, is needed (pocr_tree_attention_workspace)", (long long)need);
     OnDevice dev;
     if (dev.enter(device_id)) return 1;
     TreeAttnArgs a{t->q, c->k, c->v, c->k_exp, c->v_exp, t->page_table, t->lengths, t->q_start, t->mask, t->out, t->lse, static_cast<float *>(t->workspace),
                    t->q_token_stride, t->q_head_stride, t->page_table_stride, t->mask_stride, t->tokens, t->seqs, t->heads, c->kv_heads, c->num_pages, page_shift(c),
-                   t->max_pages, t->mask_words, t->zero_rest, p.nsplit, p.tiles, (uint32_t)p.slots, (uint32_t)p.run, t->scale};
+                   t->max_pages, t->mask_words, t->zero_rest, p.nsplit, p.tiles, (uint32_t)p.slots, (uint32_t)p.run, (uint32_t)p.part_rows,
+                   (uint32_t)p.tile_rows, t->scale};
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         return c->format == POCR_KV_FP8 ? attend_by_dim<DT, KV_FP8>(c->head_dim, p, stream, a) : attend_by_dim<DT, KV_BF16>(c->head_dim, p, stream, a);

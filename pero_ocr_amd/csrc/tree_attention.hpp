@@ -48,12 +48,18 @@ struct TreeAttnArgs {
     const uint64_t *mask;
     void *out;
     float *lse;
-    float *part;                  // nsplit > 1: averages [nsplit][tokens * heads][D], then (maximum, sum) [nsplit][tokens * heads][2]
+    float *part;                  // nsplit > 1: averages [nsplit][part_rows][D], then (maximum, sum) [nsplit][part_rows][2]
     int64_t q_ts, q_hs, table_stride, mask_stride, tokens;
     int32_t seqs, heads, kv_heads, num_pages, page_shift, max_pages, mask_words, zero_rest, nsplit, tiles;
-    uint32_t slots, run;
+    uint32_t slots, run, part_rows, tile_rows;
     float scale;
 };
+
+// Row of `part` for row r of a sequence and key head: that of the output (tile_rows = 0), or, where that is fewer rows (padding behind the last sequence
+// has none then), `tile_rows` for each sequence and key head.
+__device__ __forceinline__ uint32_t part_row(const TreeAttnArgs &a, int s, int hk, uint32_t r, int64_t to) {
+    return a.tile_rows ? ((uint32_t)s * (uint32_t)a.kv_heads + (uint32_t)hk) * a.tile_rows + r : (uint32_t)to;
+}
 
 // arrays that no kernel of the call writes, read by a whole wave at one place: through the scalar cache
 typedef const __attribute__((address_space(4))) int32_t *ScalarInts;
@@ -350,10 +356,14 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
     const uint32_t qkeep = c == 0.f ? 0u : ~0u, qflip = c < 0.f ? 0x80008000u : 0u;          // the same for bfloat16 queries, on the bits
 
     const int32_t blocks = (int32_t)(((uint32_t)sq.len + 31u) >> 5), per = (int32_t)(((uint32_t)blocks + a.nsplit - 1u) / (uint32_t)a.nsplit);
-    const int32_t first_block = min(split * per, blocks), end_block = min(first_block + per, blocks);
     const int32_t ctx = sq.len - sq.n;
 
-    for (uint32_t r0 = tile0 * (16 * RT); r0 < rows; r0 += a.tiles ? (uint32_t)a.tiles * (16 * RT) : rows) {
+    // (a second turn: the sequence has more new tokens than the caller said.  With tile_rows their splits have no room in `part`: the splits' workgroups
+    // take whole tiles in turn)
+    for (uint32_t r0 = tile0 * (16 * RT), turn = 0; r0 < rows; r0 += a.tiles ? (uint32_t)a.tiles * (16 * RT) : rows, ++turn) {
+        const bool whole_tile = turn > 0 && a.tile_rows > 0;
+        if (whole_tile && (turn - 1) % (uint32_t)a.nsplit != (uint32_t)split) continue;
+        const int32_t first_block = whole_tile ? 0 : min(split * per, blocks), end_block = whole_tile ? blocks : min(first_block + per, blocks);
         int32_t tok[RT];
         int64_t at[RT];                                               // row of out, -1: none
         Frag q[RT][ST][QP];
@@ -604,10 +614,11 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
 #pragma unroll
             for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const ta_f32x4 *>(&osum[w][rr][d]);
             const float mc = whole[rr][0], ll = whole[rr][1];
-            if (a.nsplit > 1) {
-                *reinterpret_cast<ta_f32x4 *>(a.part + ((int64_t)split * a.tokens * a.heads + to) * D + d) = v;
+            if (a.nsplit > 1 && !whole_tile) {
+                const int64_t pr = (int64_t)split * a.part_rows + part_row(a, s, hk, r0 + (uint32_t)rr, to);
+                *reinterpret_cast<ta_f32x4 *>(a.part + pr * D + d) = v;
                 if (d == 0) {
-                    float *ml = a.part + (int64_t)a.nsplit * a.tokens * a.heads * D + ((int64_t)split * a.tokens * a.heads + to) * 2;
+                    float *ml = a.part + (int64_t)a.nsplit * a.part_rows * D + pr * 2;
                     ml[0] = ll == 0.f ? -INFINITY : mc;
                     ml[1] = ll;
                 }
@@ -634,11 +645,9 @@ __global__ __launch_bounds__(256) void tree_attention_join_kernel(TreeAttnArgs a
     using T = typename ElemOf<DT>::type;
     constexpr int E = D < 64 ? 1 : D / 64;                            // neighbouring elements of a lane
     const int lane = threadIdx.x & 63;
-    const uint32_t total = (uint32_t)a.tokens * (uint32_t)a.heads, at = blockIdx.x * 4 + (threadIdx.x >> 6);
+    // grid: tile_rows / 4, key heads, sequences; or all rows / 4
+    const uint32_t total = a.part_rows, r = blockIdx.x * 4 + (threadIdx.x >> 6), at = (blockIdx.z * (uint32_t)a.kv_heads + blockIdx.y) * a.tile_rows + r;
     if (at >= total) return;
-    const int32_t token = (int32_t)(at / (uint32_t)a.heads);
-    const ScalarInts starts = (ScalarInts)a.starts;
-    if (token < starts[0] || token >= starts[a.seqs]) return;
     const float *ml = a.part + (int64_t)a.nsplit * total * D + (int64_t)at * 2;
     float ms[2], ls[2];                                               // splits lane and lane + 64
 #pragma unroll
@@ -646,6 +655,17 @@ __global__ __launch_bounds__(256) void tree_attention_join_kernel(TreeAttnArgs a
         const int s = lane + 64 * i;
         ms[i] = s < a.nsplit ? ml[(int64_t)s * total * 2] : -INFINITY;
         ls[i] = s < a.nsplit ? ml[(int64_t)s * total * 2 + 1] : 0.f;
+    }
+    int64_t to = at;                                                  // row of out
+    if (a.tile_rows) {                                                // (asked behind the loads above, which stay within `part` also where the row is nobody's)
+        const uint32_t group = (uint32_t)a.heads / (uint32_t)a.kv_heads, tok = r / group;
+        const TreeSeq sq = tree_seq(a, (int)blockIdx.z);
+        if (tok >= (uint32_t)sq.n) return;
+        to = (int64_t)(sq.first + (int32_t)tok) * a.heads + blockIdx.y * group + (r - tok * group);
+    } else {
+        const int32_t token = (int32_t)(at / (uint32_t)a.heads);
+        const ScalarInts starts = (ScalarInts)a.starts;
+        if (token < starts[0] || token >= starts[a.seqs]) return;
     }
     float m = fmaxf(ms[0], ms[1]);
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -678,12 +698,12 @@ __global__ __launch_bounds__(256) void tree_attention_join_kernel(TreeAttnArgs a
     };
     if (a.nsplit <= 4) add(std::integral_constant<int, 4>());
     else add(std::integral_constant<int, 16>());
-    T *out = static_cast<T *>(a.out) + (int64_t)at * D + lane * E;
+    T *out = static_cast<T *>(a.out) + to * D + lane * E;
     if (lane * E < D) {
 #pragma unroll
         for (int e = 0; e < E; ++e) out[e] = (T)(l == 0.f ? 0.f : acc[e]);
     }
-    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147180559945f;
+    if (a.lse && lane == 0) a.lse[to] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147180559945f;
 }
 
 }  // namespace pocr

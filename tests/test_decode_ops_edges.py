@@ -3,8 +3,9 @@ near the top of the range, scratch memory, tensors with tangents, a cache whose 
 import pytest
 import torch
 
-from pero_ocr_amd import decode_ops as ops
-from test_decode_ops import _check, _gen, _problem
+from oracle import decode_oracle as oracle
+from pero_ocr_amd import _native, decode_ops as ops
+from test_decode_ops import _check, _fake_pages, _gen, _problem
 
 
 @pytest.mark.gpu
@@ -54,3 +55,47 @@ def test_gpu_attention_of_large_values_all_widths(dim):
     for cache in ("bf16", "fp8"):
         p = _large(cache, "fp32", [70, 18], [20, 3], 2.9e38, 92, heads=4, kv_heads=2, dim=dim)
         _check(p, "fp32", ops.tree_attention(**p, want_lse=True))
+
+
+def test_workspace_does_not_grow_with_padding():
+    """scratch memory follows the rows that a batch can have by its own max_queries, not the rows it is padded to"""
+    lib, p = _native.load(), 1 << 20
+
+    def need(tokens, seqs, heads, kv_heads, dim, max_pages, most):
+        pages = _fake_pages(num_pages=1 << 20, kv_heads=kv_heads, head_dim=dim)
+        args = _native.TreeAttentionArgs(q=p, out=p, page_table=p, lengths=p, q_start=p, tokens=tokens, seqs=seqs, heads=heads, max_pages=max_pages, max_queries=most,
+                                         q_head_stride=dim, q_token_stride=heads * dim, dtype=1)
+        return lib.pocr_tree_attention_workspace(pages, args)
+    for seqs, heads, kv_heads, dim, most in ((4, 64, 8, 128, 1), (1, 8, 8, 256, 1), (3, 32, 8, 64, 5), (16, 8, 8, 128, 1)):
+        alone = need(seqs * most, seqs, heads, kv_heads, dim, 8192, most)
+        assert alone > 0
+        for tokens in (1024, 8192, 100000):
+            assert need(tokens, seqs, heads, kv_heads, dim, 8192, most) == alone
+    # whatever is said of them, never more than 32 MB
+    for tokens in (1, 7, 64, 1000, 30000, 1 << 20):
+        for seqs in (1, 2, 30, 500):
+            for heads, kv_heads, dim in ((1, 1, 32), (8, 8, 256), (64, 8, 128), (40, 2, 64)):
+                for most in (0, 1, 33, tokens):
+                    assert need(tokens, seqs, heads, kv_heads, dim, 1 << 16, most) <= 32 << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1, 0, 1], [3, 2, 5]])
+def test_gpu_padded_batch_costs_no_scratch_memory(counts):
+    """the same rows, padded or not, and no more memory than outputs and zeros.  (Not always the same bits: padding may leave other tiles and
+    splits, so sums in another order; what that may change is in the oracle's bounds.)"""
+    p = _problem([9000, 2000, 40], counts, 16, 2, 64, 64, "bf16", "fp8", 95, mask="tree")
+    n = sum(counts)
+    for most in (max(counts), 1):
+        want = ops.tree_attention(**p, max_queries=most, want_lse=True)
+        _check(p, "bf16", want)
+        tail = 5000
+        wide = dict(p, q=torch.cat([p["q"], torch.ones(tail, 16, 64, device="cuda", dtype=torch.bfloat16)]), mask=torch.cat([p["mask"], torch.full((tail, 1), -1, device="cuda")]))
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out, lse = ops.tree_attention(**wide, max_queries=most, want_lse=True)
+        used = torch.cuda.max_memory_allocated() - before
+        assert used <= out.numel() * 2 + lse.numel() * 4 + (32 << 20)
+        _check(p, "bf16", (out[:n], lse[:n]))
+        assert (out[n:] == 0).all() and torch.isneginf(lse[n:]).all()
