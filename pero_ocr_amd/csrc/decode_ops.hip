@@ -216,7 +216,8 @@ int64_t score_workspace(const pocr_token_logprobs_args *t) {
 // to 8 of them (500 classes, fp32: top 4 22.7 us against 33.5 by a wave that looks among the largest, top 8 32 and 35, top 20 62 and 47), and
 // with 16-bit logits, whose single loads are half as wide, only for few rows (500 classes, top 8: 48 us against 39).
 // Otherwise a wave (rows enough, and a row too short for more: 2000 classes in fp32, top 4 86 us, with 256 threads 110; 4000 classes 170 and
-// 156), 256 threads (600 rows of 1000 classes, top 20: 7.2 us, a wave 12.1), or 1024 (1024 rows of 131072 in bf16, top 20: 52.7 us, with 256
+// 156; and few enough alternatives for a threshold among the maxima of 64 lanes to leave a short list, without which every alternative is a pass over
+// the row: 16384 rows of 1200 in fp32, top 26 41.7 us and 46.8, top 28 91.7 and 47.6, top 32 377 and 48.3, top 64 734 and 57.7), 256 threads (600 rows of 1000 classes, top 20: 7.2 us, a wave 12.1), or 1024 (1024 rows of 131072 in bf16, top 20: 52.7 us, with 256
 // 67.3; 3000 rows of 32000 68.5 and 52.6).
 template <int DT> int score(void *stream, const LogprobArgs &a) {
     const char *w = "pocr_token_logprobs";
@@ -229,7 +230,7 @@ template <int DT> int score(void *stream, const LogprobArgs &a) {
     if (a.C <= 1024 && a.top <= 8 && rows <= 4096) return a.C <= 512 ? few(token_logprobs_few_kernel<DT, 64, 8>, 64) : few(token_logprobs_few_kernel<DT, 64, 16>, 64);
     if constexpr (DT == DT_F32)
         if (a.C <= 512 && a.top <= 8) return few(token_logprobs_few_kernel<DT, 16, 32>, 16);
-    if (a.C <= 2048 && rows > 2048) return row(token_logprobs_kernel<DT, 64>, 64);
+    if (a.C <= 2048 && rows > 2048 && a.top <= LP_WAVE_TOP) return row(token_logprobs_kernel<DT, 64>, 64);
     if (a.C <= 32768) return row(token_logprobs_kernel<DT, 256>, 256);
     if (a.slices == 1) return row(token_logprobs_kernel<DT, 1024>, 1024);
     if (launch(w, token_logprobs_kernel<DT, 256, true>, dim3((unsigned)(rows * a.slices)), dim3(256), stream, a)) return 1;

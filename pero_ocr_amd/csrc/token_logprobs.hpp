@@ -173,6 +173,7 @@ __global__ __launch_bounds__(256) void token_logprobs_few_kernel(LogprobArgs a) 
 // top 20 64).  So reductions stay in registers, and the list of a single wave is short: 2.6 KB of LDS let 32 of them share a CU (with 9 KB 17,
 // 52 -> 33 us for rows of 500, top 4).
 constexpr int LP_CAND = 1024, LP_SLACK = 32, LP_GRID = 1 << 21;       // (rows in the first axis of the grid)
+constexpr int LP_WAVE_TOP = 26;                                       // alternatives that a single wave picks
 constexpr int lp_cand(int threads) { return threads == 64 ? 256 : LP_CAND; }
 
 template <int DT, int V> __device__ __forceinline__ void lp_load(const void *p, float (&x)[V]) {

@@ -1,5 +1,7 @@
 """Decoding operators (pero_ocr_amd/decode_ops.py) at the edges of what their documentation allows: outputs beside a padded batch, finite values
 near the top of the range, scratch memory, tensors with tangents, a cache whose memory has moved."""
+import math
+
 import pytest
 import torch
 
@@ -99,3 +101,28 @@ def test_gpu_padded_batch_costs_no_scratch_memory(counts):
         assert used <= out.numel() * 2 + lse.numel() * 4 + (32 << 20)
         _check(p, "bf16", (out[:n], lse[:n]))
         assert (out[n:] == 0).all() and torch.isneginf(lse[n:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("classes", [520, 1000, 2048])
+def test_gpu_many_alternatives_do_not_cost_a_pass_each(classes, kind):
+    """rows by the thousand: 64 alternatives take the time of 24 times a few, not of a pass over the row for each"""
+    x = (torch.randn(16384, classes, device="cuda", generator=_gen(5)) * 3).to(kind)
+    tokens = torch.zeros(16384, dtype=torch.int64, device="cuda")
+
+    def time(top):
+        ops.token_logprobs(x, tokens, top=top)
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(5):
+                ops.token_logprobs(x, tokens, top=top)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+    few = time(24)
+    for top in (28, 32, 64):
+        assert time(top) <= 5 * few, top
