@@ -69,10 +69,12 @@ def test_workspace_does_not_grow_with_padding():
                                          q_head_stride=dim, q_token_stride=heads * dim, dtype=1)
         return lib.pocr_tree_attention_workspace(pages, args)
     for seqs, heads, kv_heads, dim, most in ((4, 64, 8, 128, 1), (1, 8, 8, 256, 1), (3, 32, 8, 64, 5), (16, 8, 8, 128, 1)):
-        alone = need(seqs * most, seqs, heads, kv_heads, dim, 8192, most)
-        assert alone > 0
-        for tokens in (1024, 8192, 100000):
-            assert need(tokens, seqs, heads, kv_heads, dim, 8192, most) == alone
+        alone, padded = (need(n, seqs, heads, kv_heads, dim, 8192, most) for n in (seqs * most, 1024))
+        rows = heads // kv_heads * most
+        tile = 16 if rows <= 16 else 32                                # (padded, every sequence and key head has whole tiles of rows)
+        assert 0 < alone <= padded <= alone * tile * -(-rows // tile) // rows
+        for tokens in (8192, 100000):
+            assert need(tokens, seqs, heads, kv_heads, dim, 8192, most) == padded
     # whatever is said of them, never more than 32 MB
     for tokens in (1, 7, 64, 1000, 30000, 1 << 20):
         for seqs in (1, 2, 30, 500):
