@@ -15,7 +15,8 @@ csrc/decode_ops.hip, include/pocr.h "decoding operators".  One step of a loop th
 
 Every call enqueues on torch's current stream of the tensors' device and returns; tensors made on another stream are the caller's to
 order, as for any torch operation.  Results and scratch memory come from torch's allocator, so calls may run on several streams at once
-and may be captured into graphs.  Inference only: a tensor that requires a gradient is refused while gradients are recorded.
+and may be captured into graphs.  Inference only: a tensor that requires a gradient is refused while gradients are recorded, one that carries
+a forward-mode derivative always.
 There is no CPU path.  Importing this module loads torch: it has to happen before the first engine or `_native.load()` of the process,
 because torch brings its own HIP runtime and device pointers are only valid inside one (a process that holds two is refused)."""
 from __future__ import annotations
@@ -25,6 +26,7 @@ from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _native
 
@@ -78,6 +80,11 @@ def _need(t, name: str, device: Optional[torch.device], dtypes, dims: int):
         raise RuntimeError(f"{name} requires a gradient: the decoding operators are for inference (use torch.no_grad())")
 
 
+def _no_tangent(**tensors):
+    """(called inside a level of forward-mode differentiation, _forward._current_level >= 0; such a tensor is an ordinary one by all other signs)"""
+    for name, t in tensors.items():
+        if isinstance(t, _Tensor) and _forward.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} carries a forward-mode derivative: the decoding operators are for inference")
 
 
 class KVPages:
@@ -87,6 +94,8 @@ class KVPages:
     __slots__ = ("k", "v", "k_exp", "v_exp", "index", "native")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None):
+        if _forward._current_level >= 0:
+            _no_tangent(k=k, v=v)
         fp8 = k_exp is not None
         if not (type(k) is _Tensor and type(v) is _Tensor and k.is_cuda and k.dtype is (_FP8 if fp8 else _BF16) and v.dtype is k.dtype
                 and k.dim() == 4 and k.shape == v.shape and v.get_device() == k.get_device() and k.is_contiguous() and v.is_contiguous()
@@ -151,6 +160,8 @@ def kv_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
     slots of one call are distinct."""
     tokens = _check_slots(slots, pages)
     n, index = pages.native, pages.index
+    if _forward._current_level >= 0:
+        _no_tangent(k=k, v=v)
     if not (type(k) is _Tensor and type(v) is _Tensor and k.dtype in _DTYPES and v.dtype is k.dtype and k.dim() == 3 == v.dim()
             and k.get_device() == index == v.get_device() and not (k.requires_grad or v.requires_grad)):
         _need(k, "k", pages.device, _DTYPES, 3)
@@ -172,6 +183,8 @@ def kv_read(pages: KVPages, slots: torch.Tensor, dtype: torch.dtype = torch.floa
     tokens = _check_slots(slots, pages)
     if dtype not in _DTYPES:
         raise TypeError(f"dtype {dtype}: float32, bfloat16 or float16")
+    if _forward._current_level >= 0:
+        _no_tangent(cache=pages.k, cached_values=pages.v)
     n, index = pages.native, pages.index
     k = pages.k.new_empty((tokens, n.kv_heads, n.head_dim), dtype=dtype)
     v = torch.empty_like(k)
@@ -213,6 +226,8 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
     -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros in a
     tensor made here and are left alone in an `out` of the caller's (contiguous); lse, always made here, has -inf there."""
     n, index = pages.native, pages.index
+    if _forward._current_level >= 0:
+        _no_tangent(q=q, out=out, cache=pages.k, cached_values=pages.v)
     if not (type(q) is _Tensor and type(page_table) is _Tensor and type(lengths) is _Tensor and type(q_start) is _Tensor and q.dtype in _DTYPES
             and page_table.dtype is _INT and lengths.dtype is _INT and q_start.dtype is _INT and q.dim() == 3 and page_table.dim() == 2
             and lengths.dim() == 1 and q_start.dim() == 1 and not q.requires_grad
@@ -272,6 +287,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     padding; NaN for one beyond the classes); entropy float32 [rows] of softmax(row); top_logprob float32 and top_index int32 [rows, top], the
     `top` <= 64 likeliest classes, equally likely ones in the order of their index.  A logit of -inf has probability 0; a row of nothing else
     has log probabilities -inf and entropy 0; a row with NaN or +inf has NaN."""
+    if _forward._current_level >= 0:
+        _no_tangent(logits=logits)
     if not (type(logits) is _Tensor and type(tokens) is _Tensor and logits.is_cuda and logits.dtype in _DTYPES and logits.dim() == 2 and tokens.dtype in _IDS
             and 1 <= tokens.dim() <= 2 and tokens.get_device() == logits.get_device() and not logits.requires_grad):
         _need(logits, "logits", None, _DTYPES, 2)

@@ -128,3 +128,45 @@ def test_gpu_many_alternatives_do_not_cost_a_pass_each(classes, kind):
     few = time(24)
     for top in (28, 32, 64):
         assert time(top) <= 5 * few, top
+
+
+def _dual_calls(device):
+    from torch.autograd import forward_ad
+    x = torch.ones(3, 2, 64, device=device)
+    ids = torch.zeros(3, dtype=torch.int64, device=device)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        rows = forward_ad.make_dual(x[:, 0], torch.ones_like(x[:, 0]))
+        half = torch.zeros(2, 2, 16, 64, dtype=torch.bfloat16, device=device)
+        with pytest.raises(RuntimeError, match="derivative"):
+            ops.token_logprobs(rows, ids)
+        with pytest.raises(RuntimeError, match="derivative"):
+            ops.KVPages(forward_ad.make_dual(half, half.clone()), half.clone())
+        if device == "cuda":
+            pages = ops.kv_pages(2, 2, 16, 64)
+            plain = x.clone()
+            for k, v in ((dual, plain), (plain, dual)):
+                with pytest.raises(RuntimeError, match="derivative"):
+                    ops.kv_write(pages, k, v, ids)
+            p = _problem([20], [3], 2, 2, 64, 16, "fp32", "fp8", 1)
+            with pytest.raises(RuntimeError, match="derivative"):
+                ops.tree_attention(**dict(p, q=dual))
+            with pytest.raises(RuntimeError, match="derivative"):
+                ops.tree_attention(**p, out=dual)
+            cache = ops.kv_pages(2, 2, 16, 64, dtype="bf16")
+            cache.k.copy_(forward_ad.make_dual(half, torch.ones_like(half)))          # (the tangent comes with the numbers)
+            for call in (lambda: ops.kv_read(cache, ids), lambda: ops.tree_attention(**dict(p, pages=cache))):
+                with pytest.raises(RuntimeError, match="derivative"):
+                    call()
+            ops.tree_attention(**p)                                    # (tensors without a tangent, inside the level)
+            ops.token_logprobs(x[:, 0], ids)
+
+
+def test_tangents_are_refused():
+    """forward-mode derivatives: refused as gradients are, not dropped in silence"""
+    _dual_calls("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_tangents_are_refused():
+    _dual_calls("cuda")
