@@ -22,6 +22,7 @@ because torch brings its own HIP runtime and device pointers are only valid insi
 from __future__ import annotations
 
 import ctypes as C
+from operator import attrgetter
 from typing import Optional, Sequence, Tuple
 
 import numpy as np
@@ -90,8 +91,11 @@ def _no_tangent(**tensors):
 class KVPages:
     """One layer's cache: k, v [pages, kv_heads, page_size, head_dim], bfloat16 or float8_e4m3fn; in 8 bits k_exp, v_exp uint8
     [pages, kv_heads, page_size] hold the power of two of every row: it stands for code * 2 ** (exp - 127).  Slot s is row
-    s % page_size of page s // page_size.  The tensors stay the caller's (contiguous, same device); kv_pages() makes them."""
-    __slots__ = ("k", "v", "k_exp", "v_exp", "index", "native")
+    s % page_size of page s // page_size.  The tensors stay the caller's (contiguous, same device); kv_pages() makes them.  They are read-only
+    attributes and have to keep their memory: a call with a cache whose tensors were given other storage is refused."""
+    __slots__ = ("_k", "_v", "_k_exp", "_v_exp", "_index", "_native", "_at")
+    k, v, k_exp, v_exp = (property(attrgetter(name)) for name in __slots__[:4])
+    index, native = property(attrgetter("_index")), property(attrgetter("_native"))
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None):
         if _forward._current_level >= 0:
@@ -111,8 +115,16 @@ class KVPages:
             raise ValueError(f"page_size {p}: a power of two from 16 on")
         if n < 1 or h < 1:
             raise ValueError(f"an empty cache: {tuple(k.shape)}")
-        self.k, self.v, self.k_exp, self.v_exp, self.index = k, v, k_exp, v_exp, k.get_device()
-        self.native = _native.KvPages(k.data_ptr(), v.data_ptr(), k_exp.data_ptr() if fp8 else None, v_exp.data_ptr() if fp8 else None, n, h, p, d, fp8)
+        at = (k.data_ptr(), v.data_ptr(), k_exp.data_ptr() if fp8 else None, v_exp.data_ptr() if fp8 else None)
+        self._k, self._v, self._k_exp, self._v_exp, self._index, self._at = k, v, k_exp, v_exp, k.get_device(), at
+        self._native = _native.KvPages(*at, n, h, p, d, fp8)
+
+    def plan(self) -> _native.KvPages:
+        """The cache as the C entries take it; raises if a tensor is no longer where it was when this object was made."""
+        k, v, k_exp, v_exp = self._at
+        if self._k.data_ptr() != k or self._v.data_ptr() != v or k_exp is not None and (self._k_exp.data_ptr() != k_exp or self._v_exp.data_ptr() != v_exp):
+            raise RuntimeError("the cache's tensors have other memory than when this KVPages was made: make a new one")
+        return self._native
 
     @property
     def device(self) -> torch.device:
@@ -147,7 +159,7 @@ def kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype
 
 
 def _check_slots(slots, pages: KVPages) -> int:
-    if not (type(slots) is _Tensor and slots.dtype in _IDS and slots.dim() == 1 and slots.get_device() == pages.index):
+    if not (type(slots) is _Tensor and slots.dtype in _IDS and slots.dim() == 1 and slots.get_device() == pages._index):
         _need(slots, "slots", pages.device, _IDS, 1)
     if not slots.is_contiguous():
         raise ValueError("slots must be contiguous")
@@ -159,7 +171,7 @@ def kv_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
     projection) into the cache's format and stores them at slots [tokens].  A slot outside the cache (-1 for padding) is skipped; the
     slots of one call are distinct."""
     tokens = _check_slots(slots, pages)
-    n, index = pages.native, pages.index
+    n, index = pages.plan(), pages._index
     if _forward._current_level >= 0:
         _no_tangent(k=k, v=v)
     if not (type(k) is _Tensor and type(v) is _Tensor and k.dtype in _DTYPES and v.dtype is k.dtype and k.dim() == 3 == v.dim()
@@ -185,7 +197,7 @@ def kv_read(pages: KVPages, slots: torch.Tensor, dtype: torch.dtype = torch.floa
         raise TypeError(f"dtype {dtype}: float32, bfloat16 or float16")
     if _forward._current_level >= 0:
         _no_tangent(cache=pages.k, cached_values=pages.v)
-    n, index = pages.native, pages.index
+    n, index = pages.plan(), pages._index
     k = pages.k.new_empty((tokens, n.kv_heads, n.head_dim), dtype=dtype)
     v = torch.empty_like(k)
     if _lib().pocr_kv_read(index, _stream(index), n, slots.data_ptr(), slots.dtype is _LONG, tokens, k.data_ptr(), v.data_ptr(), _DTYPES[dtype]):
@@ -225,7 +237,7 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
 
     -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros in a
     tensor made here and are left alone in an `out` of the caller's (contiguous); lse, always made here, has -inf there."""
-    n, index = pages.native, pages.index
+    n, index = pages.plan(), pages._index
     if _forward._current_level >= 0:
         _no_tangent(q=q, out=out, cache=pages.k, cached_values=pages.v)
     if not (type(q) is _Tensor and type(page_table) is _Tensor and type(lengths) is _Tensor and type(q_start) is _Tensor and q.dtype in _DTYPES

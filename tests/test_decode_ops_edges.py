@@ -170,3 +170,50 @@ def test_tangents_are_refused():
 @pytest.mark.gpu
 def test_gpu_tangents_are_refused():
     _dual_calls("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp8", "bf16"])
+def test_gpu_cache_tensors_stay(dtype):
+    """the tensors of a cache cannot be exchanged"""
+    pages = ops.kv_pages(4, 2, 16, 64, dtype=dtype)
+    for name in ("k", "v", "k_exp", "v_exp", "index", "native"):
+        with pytest.raises(AttributeError):
+            setattr(pages, name, getattr(pages, name))
+        with pytest.raises(AttributeError):
+            delattr(pages, name)
+
+
+def _as_if(monkeypatch, dtype):
+    """a KVPages of CPU tensors, past the check of the device: what is looked at before anything is enqueued"""
+    monkeypatch.setattr(ops.KVPages, "_refuse", staticmethod(lambda *a: None))
+    shape = (4, 2, 16, 64)
+    if dtype == "bf16":
+        return ops.KVPages(*(torch.zeros(shape, dtype=torch.bfloat16) for _ in range(2)))
+    return ops.KVPages(*(torch.zeros(shape, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)), *(torch.zeros(shape[:3], dtype=torch.uint8) for _ in range(2)))
+
+
+@pytest.mark.parametrize("dtype, name", [("bf16", "k"), ("bf16", "v"), ("fp8", "k"), ("fp8", "v"), ("fp8", "k_exp"), ("fp8", "v_exp")])
+def test_cache_that_has_moved_is_refused(monkeypatch, dtype, name):
+    """other storage under a tensor of the cache: every call raises before the library sees a pointer"""
+    def never(*a):
+        raise AssertionError("the library was called")
+    monkeypatch.setattr(ops, "_lib", never)
+    for how in ("data", "set_", "freed"):
+        pages = _as_if(monkeypatch, dtype)
+        assert pages.plan() is pages.native
+        t = getattr(pages, name)
+        keep = t.untyped_storage()                                     # (its memory stays taken: the new one lies elsewhere)
+        if how == "data":
+            t.data = torch.empty_like(t)
+        elif how == "set_":
+            t.set_(torch.empty_like(t))
+        else:
+            keep.resize_(0)
+        x = torch.zeros(3, 2, 64)
+        ids = torch.zeros(3, dtype=torch.int64)
+        one = torch.ones(1, dtype=torch.int32)
+        for call in (pages.plan, lambda: ops.kv_write(pages, x, x, ids), lambda: ops.kv_read(pages, ids),
+                     lambda: ops.tree_attention(x, pages, one[:, None], one, torch.tensor([0, 3], dtype=torch.int32))):
+            with pytest.raises(RuntimeError, match="other memory"):
+                call()
