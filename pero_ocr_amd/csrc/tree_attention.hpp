@@ -276,6 +276,11 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
     constexpr int QP = DT == DT_F32 ? 3 : DT == DT_F16 ? 2 : 1;      // planes of the query
     constexpr int PP = DT == DT_F32 ? 3 : 2;                         // planes of the probabilities
     constexpr int NB = D / 16, ST = D / 32, TW = Block::TW;
+    // The low plane of a float16 query lies in LDS, the same for all waves, where two tiles of 128 would not fit the registers of two waves a SIMD with it
+    // (13 to 24 of them went to scratch memory).
+    constexpr bool QLOW = DT == DT_F16 && RT == 2 && D == 128;
+    constexpr int QR = QLOW ? 1 : QP;                                // planes in registers
+    __shared__ kv_u32x4 qlow[QLOW ? RT * ST * 64 : 1];
     const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     constexpr int PITCH = D + 4;                                      // (16 rows, four words each: all 64 banks)
@@ -366,7 +371,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
         const int32_t first_block = whole_tile ? 0 : min(split * per, blocks), end_block = whole_tile ? blocks : min(first_block + per, blocks);
         int32_t tok[RT];
         int64_t at[RT];                                               // row of out, -1: none
-        Frag q[RT][ST][QP];
+        Frag q[RT][ST][QR];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const uint32_t r = r0 + 16 * rt + row, rr = min(r, rows - 1);
@@ -385,10 +390,16 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                     load_row<DT, true>(qr + Block::key_elem(g, st), x);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] *= csign;
-                    split_planes<QP>(x, q[rt][st]);
+                    if constexpr (QLOW) {
+                        Frag f[QP];
+                        split_planes<QP>(x, f);
+                        q[rt][st][0] = f[0];
+                        if (wave == 0) qlow[(rt * ST + st) * 64 + lane] = *reinterpret_cast<const kv_u32x4 *>(f[1].u);
+                    } else split_planes<QP>(x, q[rt][st]);
                 }
             }
         }
+        if constexpr (QLOW) __syncthreads();
 
         ta_f32x4 o[RT][NB];
         float m[RT], l[RT];                                           // m: of the raw scores (x csign); l: this lane's keys only
@@ -447,13 +458,22 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 ta_f32x4 sc[RT][2];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = (ta_f32x4){0.f, 0.f, 0.f, 0.f};
+                uint32_t low_at = lane;
+                if constexpr (QLOW) asm volatile("" : "+v"(low_at));  // (or it would be read ahead of the loop, into registers again)
                 if constexpr (Block::STAGED) {
                     wave_order();
                     kv.stage_keys(stage, lane);
                     wave_order();
                 }
 #pragma unroll
-                for (int c = 0; c < Block::PIECES; ++c)
+                for (int c = 0; c < Block::PIECES; ++c) {
+                    Frag low[Block::STEPS][RT];
+                    if constexpr (QLOW) {
+#pragma unroll
+                        for (int st = 0; st < Block::STEPS; ++st)
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) *reinterpret_cast<kv_u32x4 *>(low[st][rt].u) = qlow[(rt * ST + c * Block::STEPS + st) * 64 + low_at];
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         Frag kf[Block::STEPS];
@@ -461,11 +481,14 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
 #pragma unroll
                         for (int st = 0; st < Block::STEPS; ++st)
 #pragma unroll
-                            for (int rt = 0; rt < RT; ++rt)
+                            for (int rt = 0; rt < RT; ++rt) {
+                                if constexpr (QLOW) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[st].b, low[st][rt].b, sc[rt][h], 0, 0, 0);
 #pragma unroll
-                                for (int pl = QP - 1; pl >= 0; --pl)
+                                for (int pl = QR - 1; pl >= 0; --pl)
                                     sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[st].b, q[rt][c * Block::STEPS + st][pl].b, sc[rt][h], 0, 0, 0);
+                            }
                     }
+                }
                 kv.load_keys(a, next, lane);
                 page_ids(b + 2 * NW, ids);                            // (not earlier: a wait for LDS is one for these too)
                 float p[RT][8];

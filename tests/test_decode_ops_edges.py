@@ -1,13 +1,17 @@
 """Decoding operators (pero_ocr_amd/decode_ops.py) at the edges of what their documentation allows: outputs beside a padded batch, finite values
 near the top of the range, scratch memory, tensors with tangents, a cache whose memory has moved."""
 import math
+import os
+import re
+import subprocess
+import sys
+import tempfile
 
 import pytest
 import torch
 
-from oracle import decode_oracle as oracle
 from pero_ocr_amd import _native, decode_ops as ops
-from test_decode_ops import _check, _fake_pages, _gen, _problem
+from test_decode_ops import REPO, _check, _fake_pages, _gen, _problem
 
 
 @pytest.mark.gpu
@@ -217,3 +221,26 @@ def test_cache_that_has_moved_is_refused(monkeypatch, dtype, name):
                      lambda: ops.tree_attention(x, pages, one[:, None], one, torch.tensor([0, 3], dtype=torch.int32))):
             with pytest.raises(RuntimeError, match="other memory"):
                 call()
+
+
+def test_no_kernel_of_any_unit_spills():
+    """test_host.py's rule for the whole library: scratch memory per lane is 0 for every kernel of every translation unit"""
+    sys.path.insert(0, os.path.join(REPO, "tools"))
+    try:
+        from codeobj_hash import code_objects
+    finally:
+        sys.path.pop(0)
+    tool = "/opt/rocm/lib/llvm/bin/llvm-readelf"
+    if not os.path.exists(tool):
+        pytest.skip("llvm-readelf is not here")
+    seen = {}
+    for elf in code_objects(_native.lib_path()):
+        with tempfile.NamedTemporaryFile(suffix=".co") as f:
+            f.write(elf)
+            f.flush()
+            notes = subprocess.run([tool, "--notes", f.name], capture_output=True, text=True, check=True).stdout
+        for block in notes.split("- .agpr_count:")[1:]:
+            seen[re.search(r"\.symbol:\s*(\S+)", block).group(1)] = int(re.search(r"\.private_segment_fixed_size:\s*(\d+)", block).group(1))
+    for kernel in ("tree_attention_kernel", "token_logprobs_kernel", "kv_write_kernel", "ctc"):
+        assert any(kernel in name for name in seen), kernel
+    assert [name for name, size in seen.items() if size] == []
