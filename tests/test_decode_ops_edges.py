@@ -244,3 +244,18 @@ def test_no_kernel_of_any_unit_spills():
     for kernel in ("tree_attention_kernel", "token_logprobs_kernel", "kv_write_kernel", "ctc"):
         assert any(kernel in name for name in seen), kernel
     assert [name for name, size in seen.items() if size] == []
+
+
+def test_tools_see_every_code_object():
+    """the tools that read the built library's kernels read those of every translation unit"""
+    tool = "/opt/rocm/lib/llvm/bin/llvm-readelf"
+    if not os.path.exists(tool):
+        pytest.skip("llvm-readelf is not here")
+    tools = os.path.join(REPO, "tools")
+    hashes = subprocess.run([sys.executable, os.path.join(tools, "codeobj_hash.py")], capture_output=True, text=True, check=True).stdout
+    assert len(hashes.splitlines()) == len(__import__("__graft_entry__").SOURCES)
+    names = subprocess.run([sys.executable, "-c", "import codeobj_hash as c, sys; print(*c.kernels(sys.argv[1]))", _native.lib_path()], cwd=tools, capture_output=True,
+                           text=True, check=True).stdout
+    meta = subprocess.run([sys.executable, os.path.join(tools, "kernel_meta.py")], capture_output=True, text=True, check=True).stdout
+    for kernel in ("tree_attention_kernel", "token_logprobs_kernel", "kv_write_kernel", "ctc"):
+        assert kernel in names and kernel in meta, kernel
