@@ -310,11 +310,7 @@ __device__ __forceinline__ void conv_epilogue_staged(const f32x4 (&acc)[TH * MWW
             // a VALU write of a data register behind a store; tests/test_host.py::test_no_kernel_has_the_store_data_hazard scans every
             // kernel of the built library for the pair.  Loads masked by the mark - the halo's zero padding - have no data registers to
             // lose and read zeros.  profiles/r06_store_hazard.txt.
-#if POCR_EPI_MASKED_STORE        // (tools/masked_store_repro.sh builds this variant into tools/bin to study the effect; never shipped)
-            __builtin_amdgcn_raw_buffer_store_b128(val, yrsrc, (int)(ok ? (unsigned)(row * Wout + col) * pix_bytes + (unsigned)unit * 16u : kOut), (int)tile_off, 0);
-#else
             if (ok) __builtin_amdgcn_raw_buffer_store_b128(val, yrsrc, (int)((unsigned)(row * Wout + col) * pix_bytes + (unsigned)unit * 16u), (int)tile_off, 0);
-#endif
         }
         __syncthreads();                                             // (the staging area is the next tile's A buffer again)
 }

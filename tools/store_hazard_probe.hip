@@ -1,8 +1,8 @@
 // store_hazard_probe.hip - does gfx950 need a wait state between `buffer_store_dwordx4 ... sN offen` (SGPR offset) and a VALU write
 // of the store's data registers?
 //
-// Why: the library variant whose staged conv epilogue masks out-of-image lanes by an out-of-range offset instead of a branch
-// (tools/masked_store_repro.sh) gives wrong DWORDS in its own output under load (tools/three_in_flight.py: runs of two f16 channels,
+// Why: a staged conv epilogue that masks out-of-image lanes by an out-of-range offset instead of a branch
+// (a variant of the library, no longer built) gives wrong DWORDS in its own output under load (tools/three_in_flight.py: runs of two f16 channels,
 // sometimes in the high plane).  Its ISA differs from the shipped (branching) one in one respect that matters: the scheduler put
 //       buffer_store_dwordx4 v[2:5], v22, s[4:7], s11 offen
 //       v_lshrrev_b32_e32 v2, 5, v1                              <- VALU write of data register 0, zero wait states

@@ -4,8 +4,7 @@ in another launch's activations, only with three launches in flight, only in the
     python tools/three_in_flight.py [trials=6] [--prealloc] [--detail]        exit code 1 if any trial differs
 --prealloc: every slot first runs its lines ALONE (all activation buffers exist at their final size before three launches share the
 GPU) - separates "three launches in flight" from "device memory is allocated while other launches run"; --detail: where the
-differing values lie (runs of consecutive channels, magnitudes).  POCR_TMP_LIB=<path>: a variant build of the library
-(tools/masked_store_repro.sh builds the one with round 5's masked stores)."""
+differing values lie (runs of consecutive channels, magnitudes).  POCR_TMP_LIB=<path>: a variant build of the library."""
 import os
 import sys
 
