@@ -409,8 +409,9 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const 
  * page_table[s * page_table_stride + p / page_size]; its new tokens are rows q_start[s] .. q_start[s + 1] - 1 of q, n of them, and their keys and
  * values are already in the cache at the last n positions.  New token i sees all positions before these, and of these
  *   mask NULL : 0 .. i (a chain);   else bit j of mask row i (words of 64 bits: bit j % 64 of word j / 64, row stride mask_stride words).
- * A row whose mask leaves nothing gets out = 0 and lse = -inf.  Query head h reads key head h / (heads / kv_heads).
- * A position beyond the page table or whose page id is outside the cache is absent: nobody sees it and it is never read.
+ * A row whose mask leaves nothing, or only scores of -inf, gets out = 0 and lse = -inf.  Query head h reads key head h / (heads / kv_heads).
+ * A length beyond the page table counts as the table's max_pages * page_size positions (the new tokens are the last of these), a negative one as 0; a
+ * position whose page id is outside the cache is absent: nobody sees it and it is never read.
  * q_start is non-decreasing from 0 and ends at or below `tokens`; rows of out / lse behind q_start[seqs] are left as they were (zero_rest 0),
  * or become 0 and -inf (1), or -inf in lse while out is left alone (2).  max_queries: the most new tokens of
  * one sequence, if known (0: unknown): it shapes the launch and the workspace (at most 17 MB); any value gives the same answer but for the order of the

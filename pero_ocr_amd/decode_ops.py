@@ -231,8 +231,8 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
     cached positions, the new tokens (already written by kv_write) being the last ones; q_start int32 [seqs + 1], from 0 on.
     A new token sees every older position and, among the new ones, those up to itself (mask None) or those its mask row names (int64
     [tokens, words], see tree_mask; bits count from the sequence's first new token).  heads is a multiple of the cache's key heads;
-    query head h reads key head h // (heads // kv_heads).  A token that sees nothing gets zeros and lse -inf.  Positions whose page id
-    lies outside the cache (-1) are absent.  scale: head_dim ** -0.5 unless given.  max_queries: the most new tokens of one sequence,
+    query head h reads key head h // (heads // kv_heads).  A token that sees nothing, or only scores of -inf, gets zeros and lse -inf.
+    Positions whose page id lies outside the cache (-1) are absent; a length beyond the table counts as the table's positions.  scale: head_dim ** -0.5 unless given.  max_queries: the most new tokens of one sequence,
     if the caller knows it (it shapes the launch; the answer differs at most by the order of its sums, and comes later if there are more).
 
     -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros in a

@@ -6,6 +6,7 @@ import re
 import subprocess
 import sys
 import tempfile
+import threading
 
 import pytest
 import torch
@@ -259,3 +260,130 @@ def test_tools_see_every_code_object():
     meta = subprocess.run([sys.executable, os.path.join(tools, "kernel_meta.py")], capture_output=True, text=True, check=True).stdout
     for kernel in ("tree_attention_kernel", "token_logprobs_kernel", "kv_write_kernel", "ctc"):
         assert kernel in names and kernel in meta, kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind, cache", [("fp32", "bf16"), ("bf16", "fp8"), ("fp16", "fp8")])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(2, 1, 64), (4, 1, 128), (2, 2, 32)])
+def test_gpu_long_chains(heads, kv_heads, dim, kind, cache):
+    """prompts: hundreds of new tokens, each up to itself, with and without older positions, at the borders of tiles and blocks"""
+    for lengths, counts in (([300], [300]), ([129, 417, 33], [129, 150, 1]), ([700], [257])):
+        p = _problem(lengths, counts, heads, kv_heads, dim, 32, kind, cache, 101)
+        _check(p, kind, ops.tree_attention(**p, want_lse=True))
+        _check(p, kind, ops.tree_attention(**p, max_queries=max(counts), want_lse=True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("over", [1, 40, 1 << 20])
+def test_gpu_lengths_beyond_the_table(over):
+    """a length beyond the page table counts as the positions that the table has: the new tokens are the last of these"""
+    p = _problem([64, 64], [5, 2], 2, 1, 64, 16, "fp32", "fp8", 103, mask="tree")
+    want = ops.tree_attention(**p, want_lse=True)
+    _check(p, "fp32", want)
+    got = ops.tree_attention(**dict(p, lengths=p["lengths"] + over), want_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_gpu_expanded_arguments():
+    """one table, query, mask row, key, value, or row of logits for all: strides of zero"""
+    p = _problem([70, 70, 70], [2, 2, 2], 4, 2, 64, 16, "bf16", "fp8", 105, mask="tree")
+    p["page_table"], p["q"], p["mask"] = p["page_table"][:1].expand(3, -1), p["q"][:1].expand(6, -1, -1), p["mask"][1:2].expand(6, -1)
+    whole = dict(p, page_table=p["page_table"].contiguous(), q=p["q"].contiguous(), mask=p["mask"].contiguous())
+    assert torch.equal(ops.tree_attention(**p), ops.tree_attention(**whole))
+    _check(whole, "bf16", ops.tree_attention(**p, want_lse=True))
+    pages, same = ops.kv_pages(2, 2, 16, 64), ops.kv_pages(2, 2, 16, 64)
+    row, ids = torch.randn(1, 2, 64, device="cuda", generator=_gen(7)), torch.arange(9, device="cuda")
+    ops.kv_write(pages, row.expand(9, -1, -1), row[:, :1].expand(9, 2, -1), ids)
+    ops.kv_write(same, row.expand(9, -1, -1).contiguous(), row[:, :1].expand(9, 2, -1).contiguous(), ids)
+    for a, b in ((pages.k, same.k), (pages.v, same.v), (pages.k_exp, same.k_exp), (pages.v_exp, same.v_exp)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for a, b in zip(ops.kv_read(pages, torch.zeros(5, dtype=torch.int64, device="cuda")), ops.kv_read(pages, ids[:1])):
+        assert torch.equal(a, b.expand_as(a))                            # the same slot again and again
+    x, t = torch.randn(1, 700, device="cuda", generator=_gen(8)), torch.arange(20, device="cuda")
+    for a, b in zip(ops.token_logprobs(x.expand(20, -1), t, top=5), ops.token_logprobs(x.expand(20, -1).contiguous(), t, top=5)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_gpu_offset_integer_arguments():
+    """lengths, q_start, slots, tokens and mask rows that start in the middle of a tensor: aligned to an element, no more"""
+    p = _problem([70, 45], [3, 2], 4, 2, 64, 16, "bf16", "fp8", 107, mask="tree")
+    want = ops.tree_attention(**p)
+    moved = {k: torch.cat([p[k][:1], p[k]])[1:] for k in ("lengths", "q_start", "mask")}
+    wide = torch.full((2, p["page_table"].shape[1] + 1), 7, dtype=torch.int32, device="cuda")
+    wide[:, 1:] = p["page_table"]
+    assert torch.equal(ops.tree_attention(**dict(p, page_table=wide[:, 1:], **moved)), want)
+    x = torch.randn(6, 300, device="cuda", generator=_gen(9))
+    for kind in (torch.int32, torch.int64):
+        t = torch.arange(7, device="cuda", dtype=kind)
+        assert torch.equal(ops.token_logprobs(x, t[1:])[0], ops.token_logprobs(x, t[1:].clone())[0])
+        for a, b in zip(ops.kv_read(p["pages"], t[1:]), ops.kv_read(p["pages"], t[1:].clone())):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_gpu_threads():
+    """calls from several threads at once, each on a stream of its own"""
+    problems = [_problem([300 + 7 * i, 2100], [3, 2], 8, 2, 64, 16, "bf16", "fp8", 110 + i, mask="tree") for i in range(4)]
+    x = torch.randn(5, 120000, device="cuda", generator=_gen(11))
+    t = torch.arange(5, device="cuda")
+    want = [[u.clone() for u in ops.tree_attention(**p, want_lse=True)] for p in problems]
+    scores = [u.clone() for u in ops.token_logprobs(x, t, top=4)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got, again = ops.tree_attention(**problems[i], want_lse=True), ops.token_logprobs(x, t, top=4)
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])) or not all(torch.equal(a, b) for a, b in zip(again, scores)):
+                    bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
+
+
+@pytest.mark.gpu
+def test_gpu_inference_mode():
+    with torch.inference_mode():
+        p = _problem([40, 21], [6, 5], 2, 1, 64, 16, "fp32", "fp8", 115, mask="tree")
+        _check(p, "fp32", ops.tree_attention(**p, want_lse=True))
+        x = torch.randn(3, 50, device="cuda")
+        assert ops.token_logprobs(x, torch.arange(3, device="cuda"), top=2)[2].shape == (3, 2)
+
+
+@pytest.mark.gpu
+def test_gpu_first_calls_of_a_process_may_be_captured():
+    """nothing has to run eagerly before a capture: the first calls of a process, recorded, replayed and compared with eager ones"""
+    code = """
+import torch
+from pero_ocr_amd import decode_ops as ops
+pages = ops.kv_pages(40, 2, 16, 64)
+k, v = (torch.randn(600, 2, 64, device="cuda") for _ in range(2))
+slots = torch.arange(600, device="cuda")
+q = torch.randn(3, 4, 64, device="cuda")
+table = torch.arange(38, device="cuda", dtype=torch.int32)[None]
+lengths, starts = torch.tensor([600], device="cuda", dtype=torch.int32), torch.tensor([0, 3], device="cuda", dtype=torch.int32)
+x, t = torch.randn(3, 120000, device="cuda"), torch.arange(3, device="cuda")
+def step():
+    ops.kv_write(pages, k, v, slots)
+    return ops.kv_read(pages, slots) + ops.tree_attention(q, pages, table, lengths, starts, want_lse=True) + ops.token_logprobs(x, t, top=3)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+for turn in range(3):
+    for o in out:
+        o.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    print("same" if all(torch.equal(a, b) for a, b in zip(out, step())) else "different", flush=True)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=100)
+    assert r.stdout.split() == ["same"] * 3, r.stdout + r.stderr
