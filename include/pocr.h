@@ -415,7 +415,7 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const 
  * q_start is non-decreasing from 0 and ends at or below `tokens`; rows of out / lse behind q_start[seqs] are left as they were (zero_rest 0),
  * or become 0 and -inf (1), or -inf in lse while out is left alone (2).  max_queries: the most new tokens of
  * one sequence, if known (0: unknown): it shapes the launch and the workspace (at most 17 MB); any value gives the same answer but for the order of the
- * sums, one below the truth later.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
+ * sums, one below the truth later.  max_pages shapes the launch too: give the pages of the longest sequence where they are known.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
 typedef struct pocr_tree_attention_args {
     const void *q;                    /* [tokens][heads][head_dim], element strides q_token_stride, q_head_stride; rows start at multiples of 16 bytes */
     void *out;                        /* [tokens][heads][head_dim] contiguous, 16-byte aligned */

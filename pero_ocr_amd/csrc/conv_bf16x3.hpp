@@ -107,8 +107,8 @@ constexpr float kF16x2Scale = 2048.0f;
 // x -> (h, l): h = f16(x), l = f16((x - h) * 2^11), round to nearest even.  (Tried: l = f16(fma(h, -2^11, 2^11 x)) on v_fma_mixlo /
 // v_fma_mixhi in inline asm, 8 instead of 12 vector instructions per four values, bit-identical in isolation - but the compiler does
 // not track the sub-dword write hazard of those instructions inside an asm block: next to stores the results were right, an MFMA that
-// consumed them at once read stale low planes (the recurrence lost its l plane); written in C++ the compiler picks v_pk_fma_f32 and
-// the same 12 instructions.  No measurable time in any layer either way: dropped.)
+// consumed them at once read stale low planes (the recurrence lost its l plane); written in C++ the compiler picked v_pk_fma_f32, which
+// the build no longer allows, and the same 12 instructions.  No measurable time in any layer either way: dropped.)
 __device__ __forceinline__ void split2_quad(const f32x4 p, u32x2 &hi, u32x2 &lo) {
     const f32x2 a = {p[0], p[1]}, b = {p[2], p[3]};
     const f16x2 ha = __builtin_convertvector(a, f16x2), hb = __builtin_convertvector(b, f16x2);       // round to nearest even

@@ -127,6 +127,9 @@ AttendPlan attend_plan(const pocr_kv_pages *c, const pocr_tree_attention_args *t
     // heads of 128, 8 query heads each; in brackets the rule's: 500 keys [1] 8.6 us, 2 splits 10.0; 2000 keys 1 split 17.3, 3 12.9, [6] 11.4;
     // 8 sequences of 4000 keys 1 split 29.8, 2 21.8, [4] 19.0, 6 20.6; 32 sequences [1] 47, 2 49).  Two workgroups on each where a split still is
     // 256 blocks, so that sequences of different lengths end together (60 to 131 thousand keys: 256 workgroups 186 us, 512 169 us, 768 172 us).
+    // The lengths are on the device: the table's width stands for them.  In a table of 131072 positions one sequence of 500 keys takes 10.5 to 11 us (its
+    // own width 8.5), of 2000 keys 10.7 to 11.2 (11.4), 8 of 500 keys 11.0 to 11.9 (8.6), 8 of 4000 keys 19.5 (19.1): where one split is best the join's
+    // launch is lost, elsewhere more splits do as well.  A caller who knows the lengths passes the table's first columns.
     p.nsplit = (int)std::min<int64_t>(std::max({std::min(256 / units, blocks / 10), std::min(512 / units, blocks / 256), (int64_t)1}), TA_MAX_SPLITS);
     // Room for the splits of the rows that the slots hold (units * nsplit <= 512: at most 17 MB), not of all that a batch is padded to.
     p.tile_rows = p.tiles * (int64_t)(16 * p.rt);
@@ -198,8 +201,9 @@ int check_scores(const pocr_token_logprobs_args *t) {
 }
 
 // Workgroups of a row: more than one where rows are too few to fill the chip and so long that one workgroup (36 GB/s) takes longer than
-// the second launch and the join (9 rows of 151003 in fp32, top 8: whole 16.0 us, in slices 11.6; 64 of 152000 in bf16 16.1 and 12.9; 8 of 80000,
-// top 5, 11.5 and 10.6, top 64 13.7 and 15.7; 100 of 152000 19.5 and 19.2), up to four on each CU (64 rows of 400000 in fp32: 256 workgroups 41 us,
+// the second launch and the join (time on the GPU: 9 rows of 151003 in fp32, top 8: whole 16.0 us, in slices 11.6; 64 of 152000 in bf16 16.1 and 12.9;
+// 100 of 152000 19.5 and 19.2.  Between 65536 and 98304 classes it depends on top: 8 rows of 80000, top 5, 11.5 and 10.6, top 64 13.7 and 15.7;
+// there a row stays whole, which needs no scratch memory), up to four on each CU (64 rows of 400000 in fp32: 256 workgroups 41 us,
 // 512 28.3, 1024 27.4, whole 39), of 8192 classes or more.
 int score_slices(const pocr_token_logprobs_args *t) {
     if (t->classes <= 98304 || t->rows >= 128) return 1;

@@ -4,7 +4,8 @@
 //   top        = the `top` largest logits, equal ones in the order of their index (NaN ranks above everything, as in torch.argmax:
 //                the rule of ctc.hpp), with their log probabilities
 // A logit of -inf has probability 0 and adds nothing to the entropy; a row of nothing else has log probability -inf everywhere and
-// entropy 0; a row with a NaN or +inf has NaN for both.  Sums are in 32 bits.
+// entropy 0; a row with a NaN or +inf has NaN for both.  Sums are in 32 bits.  exp(d) is 2^(d / ln 2) with the product rounded once: off by
+// about |d| 2^-24 of itself, most where it is smallest; logarithms are log2 times ln 2 (error against 64 bits: 5e-8 of the results, the plain form's 8e-8).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -15,14 +15,16 @@
 // of eight keys and transposes them with byte permutes; tile c of the product then is elements c, D/16 + c, 2 D/16 + c, ... and a lane ends up with
 // D / 4 neighbouring outputs of its row.
 // 8-bit codes become bfloat16 exactly, by v_cvt_scalef32 with the key's own power of two.
-// What is rounded: the probability enters the second product as bf16 planes (cut, cut, rounded), two for 16-bit queries (2^-17 of it: one plane's 2^-9
-// would add as much error as rounding the result does) and three for float32 (2^-25); a float16 or float32 query is two or three bf16 planes (exact / 2^-25).
-// Scores, statistics and sums are float32.
+// What is rounded: the probability enters the second product as bf16 planes (cut, cut, rounded), two for 16-bit queries: at most 2^-16 of it (the first
+// cut leaves less than 2^-7, of which half a step is 2^-16; one plane's 2^-8 would add as much error as rounding the result does); three for float32
+// are exact, as are the two or three planes of a float16 or float32 query.  Scores, statistics and sums are float32.
 //
-// What bounds it (8 key heads): four sequences of 60 to 131 thousand keys of 128 in 8 bits, one token each, 169 us = 5.3 TB/s: the memory; 24 trees of
-// 28 to 256 rows over 0.5 to 9 thousand keys of 128 in bfloat16 204 us, half of it matrix instructions (two planes of the probabilities)
-// and conversions, the rest waits for the address unit; one tree of 132 rows over 4129 keys of 128 in 8 bits 18.1 us and 512 single
-// tokens over 40 to 272 keys of 64, fp32, 25 us, where a wave has 2 to 6 blocks and the start and the end of a workgroup (4 us) weigh most.
+// What bounds it (8 key heads; calls one after the other): four sequences of 60 to 131 thousand keys of 128 in 8 bits, one token each, 169 us = 5.3 TB/s: the
+// memory; 24 trees of 28 to 256 rows over 0.5 to 9 thousand keys of 128 in bfloat16 200 us, half of it matrix instructions (two planes of the
+// probabilities) and conversions, which every wave repeats for its 32 rows, the rest waits for the address unit; one tree of 132 rows over 4129 keys of
+// 128 in 8 bits 18.3 us (5 or 6 blocks a wave, one on its way at a time) and 512 single tokens over 40 to 272 keys of 64, fp32, 25 us (2 to 9 blocks
+// a wave), where the start and the end of a workgroup (4 us) weigh most.  A chain takes all blocks of its sequence for every row tile and masks what lies
+// behind the tile's own tokens: 2048 new tokens, nothing before them, 32 heads over 8 of 128, 138 us for 57 us of products, of which the mask leaves half.
 //
 // A NaN or infinity in V spreads in a matrix product to the masked rows, whose probability is 0; testing every element for it costs more than the
 // transposition, so the loop does not.  Finite values near the end of the range may pass it in a sum of up to 2^8 times each, where the

@@ -6,16 +6,17 @@ one launch) and the logit operators `_native.ctc_greedy` / `_native.sparsify`, f
 csrc/decode_ops.hip, include/pocr.h "decoding operators".  One step of a loop that drafts a tree of tokens and verifies it:
 
     pages = kv_pages(num_pages, kv_heads, page_size, head_dim)       # once per layer
-    mask = tree_mask(parents, device="cuda")                         # which drafted tokens each of them sees
+    mask = tree_mask(parents, device="cuda")                         # which drafted tokens each of them sees (once per form of a tree)
     kv_write(pages, k, v, slots)                                     # the drafted tokens' keys and values
     x = tree_attention(q, pages, page_table, lengths, q_start, mask=mask)
     ...                                                              # rest of the network -> logits of every drafted token
     logprob, entropy, top_logprob, top_index = token_logprobs(logits, drafted, top=8)
     kv_write(pages, k[accepted], v[accepted], next_slots)            # the accepted path moves together; lengths shrink to it
 
-Every call enqueues on torch's current stream of the tensors' device and returns; tensors made on another stream are the caller's to
+Every call but tree_mask enqueues on torch's current stream of the tensors' device and returns; tensors made on another stream are the caller's to
 order, as for any torch operation.  Results and scratch memory come from torch's allocator, so calls may run on several streams at once
-and may be captured into graphs.  Inference only: a tensor that requires a gradient is refused while gradients are recorded, one that carries
+and may be captured into graphs.  tree_mask builds a mask on the host and copies it, which waits: trees of a fixed form are made once, before the loop.
+  Inference only: a tensor that requires a gradient is refused while gradients are recorded, one that carries
 a forward-mode derivative always.
 There is no CPU path.  Importing this module loads torch: it has to happen before the first engine or `_native.load()` of the process,
 because torch brings its own HIP runtime and device pointers are only valid inside one (a process that holds two is refused)."""
@@ -207,7 +208,8 @@ def kv_read(pages: KVPages, slots: torch.Tensor, dtype: torch.dtype = torch.floa
 
 def tree_mask(parents: Sequence[int], device="cuda") -> torch.Tensor:
     """The mask of one tree of drafted tokens: parents[i] < i is the token that i continues, -1 for one that continues the cached
-    text.  -> int64 [n, ceil(n / 64)]; bit j of row i (bit j % 64 of word j // 64): token i sees token j, its ancestors and itself."""
+    text.  -> int64 [n, ceil(n / 64)]; bit j of row i (bit j % 64 of word j // 64): token i sees token j, its ancestors and itself.  Made on the
+    host, a loop over the tokens and a copy that is waited for: not for a step that is timed or captured into a graph."""
     n = len(parents)
     words = -(-n // 64)
     seen = np.zeros((n, words), dtype=np.uint64)
@@ -234,6 +236,7 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
     query head h reads key head h // (heads // kv_heads).  A token that sees nothing, or only scores of -inf, gets zeros and lse -inf.
     Positions whose page id lies outside the cache (-1) are absent; a length beyond the table counts as the table's positions.  scale: head_dim ** -0.5 unless given.  max_queries: the most new tokens of one sequence,
     if the caller knows it (it shapes the launch; the answer differs at most by the order of its sums, and comes later if there are more).
+    The table's width shapes the launch too: pass page_table[:, :n] where the longest sequence is known to have n pages.
 
     -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros in a
     tensor made here and are left alone in an `out` of the caller's (contiguous); lse, always made here, has -inf there."""
