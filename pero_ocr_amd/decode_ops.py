@@ -121,10 +121,13 @@ class KVPages:
         self._native = _native.KvPages(*at, n, h, p, d, fp8)
 
     def plan(self) -> _native.KvPages:
-        """The cache as the C entries take it; raises if a tensor is no longer where it was when this object was made."""
+        """The cache as the C entries take it; raises if a tensor is no longer where it was when this object was made, or has come to require a
+        gradient."""
         k, v, k_exp, v_exp = self._at
         if self._k.data_ptr() != k or self._v.data_ptr() != v or k_exp is not None and (self._k_exp.data_ptr() != k_exp or self._v_exp.data_ptr() != v_exp):
             raise RuntimeError("the cache's tensors have other memory than when this KVPages was made: make a new one")
+        if (self._k.requires_grad or self._v.requires_grad) and torch.is_grad_enabled():
+            raise RuntimeError("the cache requires a gradient: the decoding operators are for inference (use torch.no_grad())")
         return self._native
 
     @property

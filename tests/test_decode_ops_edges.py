@@ -387,3 +387,28 @@ for turn in range(3):
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=100)
     assert r.stdout.split() == ["same"] * 3, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("name", ["k", "v"])
+def test_cache_that_requires_a_gradient_is_refused(monkeypatch, dtype, name):
+    """also where it came to require one behind the making of the KVPages, or was made while none was recorded"""
+    def reached(*a):
+        raise ZeroDivisionError("the library was called")
+    monkeypatch.setattr(ops, "_lib", reached)
+    monkeypatch.setattr(ops, "_stream", lambda index: 0)
+    x = torch.zeros(3, 2, 64)
+    ids = torch.zeros(3, dtype=torch.int64)
+    pages = _as_if(monkeypatch, dtype)
+    with torch.no_grad():
+        getattr(pages, name).requires_grad_()
+    calls = (lambda: ops.kv_read(pages, ids), lambda: ops.kv_write(pages, x, x, ids),
+             lambda: ops.tree_attention(x, pages, *(torch.ones(s, dtype=torch.int32) for s in ((1, 1), (1,), (2,)))))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+    with torch.no_grad():
+        monkeypatch.setattr(ops, "_need", lambda *a: None)              # (past the device: without recording a call goes on to the library)
+        for call in calls:
+            with pytest.raises(ZeroDivisionError):
+                call()
