@@ -384,7 +384,8 @@ enum { POCR_F32 = 0, POCR_BF16 = 1, POCR_F16 = 2 };
  * page_size a power of two from 16 on.  Slot s = row s % page_size of page s / page_size.
  * POCR_KV_FP8: e4m3 codes; every row (one token, one head) has an exponent in k_exp / v_exp [num_pages][kv_heads][page_size] and stands
  * for code * 2^(exp - 127), exp = the smallest >= 27 with max |x| <= 448 * 2^(exp - 127).  Rounding is to nearest even: off by at most 2^-4 of
- * the value, or 2^-10 * 2^(exp - 127) below 2^-6 * 2^(exp - 127).  An element that is not finite is stored as NaN and does not count for exp.
+ * the value, or 2^-10 * 2^(exp - 127) below 2^-6 * 2^(exp - 127).  An element that is not finite is stored as NaN and does not count for exp; one of
+ * 2^128 (1 - 2^-5) or more in size is rounded to 2^128, which reads as infinity.
  * POCR_KV_BF16: rounded to nearest even; k_exp and v_exp are not used. */
 enum { POCR_KV_BF16 = 0, POCR_KV_FP8 = 1 };
 typedef struct pocr_kv_pages {
@@ -413,9 +414,10 @@ int pocr_kv_read(int device_id, void *stream, const pocr_kv_pages *pages, const 
  * A length beyond the page table counts as the table's max_pages * page_size positions (the new tokens are the last of these), a negative one as 0; a
  * position whose page id is outside the cache is absent: nobody sees it and it is never read.
  * q_start is non-decreasing from 0 and ends at or below `tokens`; rows of out / lse behind q_start[seqs] are left as they were (zero_rest 0),
- * or become 0 and -inf (1), or -inf in lse while out is left alone (2).  max_queries: the most new tokens of
- * one sequence, if known (0: unknown): it shapes the launch and the workspace (at most 17 MB); any value gives the same answer but for the order of the
- * sums, one below the truth later.  max_pages shapes the launch too: give the pages of the longest sequence where they are known.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
+ * or become 0 and -inf (1), or -inf in lse while out is left alone (2).
+ * max_queries: the most new tokens of one sequence, if known (0: unknown): it shapes the launch and the workspace (at most 17 MB); any value gives
+ * the same answer but for the order of the sums, one below the truth later.  max_pages shapes the launch too: give the pages of the longest
+ * sequence where they are known.  tokens * heads is at most 2^27, seqs * kv_heads at most 2^20.  Sums and the softmax are in 32 bits. */
 typedef struct pocr_tree_attention_args {
     const void *q;                    /* [tokens][heads][head_dim], element strides q_token_stride, q_head_stride; rows start at multiples of 16 bytes */
     void *out;                        /* [tokens][heads][head_dim] contiguous, 16-byte aligned */

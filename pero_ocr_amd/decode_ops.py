@@ -15,9 +15,9 @@ csrc/decode_ops.hip, include/pocr.h "decoding operators".  One step of a loop th
 
 Every call but tree_mask enqueues on torch's current stream of the tensors' device and returns; tensors made on another stream are the caller's to
 order, as for any torch operation.  Results and scratch memory come from torch's allocator, so calls may run on several streams at once
-and may be captured into graphs.  tree_mask builds a mask on the host and copies it, which waits: trees of a fixed form are made once, before the loop.
-  Inference only: a tensor that requires a gradient is refused while gradients are recorded, one that carries
-a forward-mode derivative always.
+and may be captured into graphs.  tree_mask builds a mask on the host and copies it, which waits: trees of a fixed form are made once, before the
+loop.  Inference only: a tensor that requires a gradient is refused while gradients are recorded, one that carries a forward-mode
+derivative always.
 There is no CPU path.  Importing this module loads torch: it has to happen before the first engine or `_native.load()` of the process,
 because torch brings its own HIP runtime and device pointers are only valid inside one (a process that holds two is refused)."""
 from __future__ import annotations
@@ -237,9 +237,10 @@ def tree_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, le
     A new token sees every older position and, among the new ones, those up to itself (mask None) or those its mask row names (int64
     [tokens, words], see tree_mask; bits count from the sequence's first new token).  heads is a multiple of the cache's key heads;
     query head h reads key head h // (heads // kv_heads).  A token that sees nothing, or only scores of -inf, gets zeros and lse -inf.
-    Positions whose page id lies outside the cache (-1) are absent; a length beyond the table counts as the table's positions.  scale: head_dim ** -0.5 unless given.  max_queries: the most new tokens of one sequence,
-    if the caller knows it (it shapes the launch; the answer differs at most by the order of its sums, and comes later if there are more).
-    The table's width shapes the launch too: pass page_table[:, :n] where the longest sequence is known to have n pages.
+    Positions whose page id lies outside the cache (-1) are absent; a length beyond the table counts as the table's positions.
+    scale: head_dim ** -0.5 unless given.  max_queries: the most new tokens of one sequence, if the caller knows it (it shapes the launch;
+    the answer differs at most by the order of its sums, and comes later if there are more).  The table's width shapes the launch too:
+    pass page_table[:, :n] where the longest sequence is known to have n pages.
 
     -> out [tokens, heads, head_dim] in q's type, or (out, lse float32 [tokens, heads]).  Rows behind q_start[-1] (a padded batch) are zeros in a
     tensor made here and are left alone in an `out` of the caller's (contiguous); lse, always made here, has -inf there."""

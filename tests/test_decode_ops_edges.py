@@ -412,3 +412,16 @@ def test_cache_that_requires_a_gradient_is_refused(monkeypatch, dtype, name):
         for call in calls:
             with pytest.raises(ZeroDivisionError):
                 call()
+
+
+@pytest.mark.gpu
+def test_gpu_rounding_at_the_end_of_the_range():
+    """half a step below 2^128 an 8-bit element is rounded to it, by the rule for all others: it reads as infinity.  Below that finite numbers stay finite"""
+    edge = 2.0 ** 128 * (1 - 2.0 ** -5)                                  # between codes 240 and 256, of which the latter is even
+    x = torch.ones(4, 1, 32, device="cuda")
+    x[0, 0, 3], x[1, 0, 3], x[2, 0, 3], x[3, 0, 3] = edge, -edge, 3.296e38, torch.finfo(torch.float32).max
+    pages = ops.kv_pages(1, 1, 16, 32)
+    ops.kv_write(pages, x, x, torch.arange(4, device="cuda"))
+    k, _v = ops.kv_read(pages, torch.arange(4, device="cuda"))
+    assert k[:, 0, 3].tolist() == [math.inf, -math.inf, 240 * 2.0 ** 120, math.inf]
+    assert pages.k_exp[0, 0, :4].tolist() == [247] * 4 and pages.k[0, 0, :4, 3].float().tolist() == [256.0, -256.0, 240.0, 256.0]
