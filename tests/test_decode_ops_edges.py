@@ -425,3 +425,23 @@ def test_gpu_rounding_at_the_end_of_the_range():
     k, _v = ops.kv_read(pages, torch.arange(4, device="cuda"))
     assert k[:, 0, 3].tolist() == [math.inf, -math.inf, 240 * 2.0 ** 120, math.inf]
     assert pages.k_exp[0, 0, :4].tolist() == [247] * 4 and pages.k[0, 0, :4, 3].float().tolist() == [256.0, -256.0, 240.0, 256.0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_gpu_attention_many_rows_all_types(dim, cache, kind):
+    """trees with more rows than one tile, in every type: two tiles a wave where they fit; in splits, in one piece, and with waves alone"""
+    p = _problem([37, 90, 33, 70], [33, 17, 20, 41], 4, 2, dim, 16, kind, cache, 121, mask="tree")
+    _check(p, kind, ops.tree_attention(**p, max_queries=41, want_lse=True))
+    p = _problem([700, 20], [33, 18], 2, 1, dim, 32, kind, cache, 122, mask="any")
+    for most in (0, 33):
+        _check(p, kind, ops.tree_attention(**p, max_queries=most, want_lse=True))
+    n = 2050                                                            # (more workgroups than two waves a SIMD: a wave each)
+    p = _problem([9] * n, [1] * n, 1, 1, dim, 16, kind, cache, 123)
+    got = ops.tree_attention(**p, max_queries=1, want_lse=True)
+    few = dict(p, q=p["q"][:40], page_table=p["page_table"][:40], lengths=p["lengths"][:40], q_start=p["q_start"][:41])
+    _check(few, kind, [t[:40] for t in got])
+    for a, b in zip(got, ops.tree_attention(**dict(p, max_queries=0), want_lse=True)):
+        assert torch.allclose(a.float(), b.float(), rtol=2 ** -7, atol=2 ** -7)          # the same sums in another order
