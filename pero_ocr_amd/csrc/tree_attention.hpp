@@ -15,8 +15,9 @@
 // of eight keys and transposes them with byte permutes; tile c of the product then is elements c, D/16 + c, 2 D/16 + c, ... and a lane ends up with
 // D / 4 neighbouring outputs of its row.
 // 8-bit codes become bfloat16 exactly, by v_cvt_scalef32 with the key's own power of two.
-// What is rounded: the probability enters the second product as bf16 planes (cut, cut, rounded), two for 16-bit queries: at most 2^-16 of it (the first
-// cut leaves less than 2^-7, of which half a step is 2^-16; one plane's 2^-8 would add as much error as rounding the result does); three for float32
+// What is rounded: the probability enters the second product as bf16 planes, two for 16-bit queries: at most 2^-17 of it (rounding to the first leaves up
+// to 2^-8, of which half a step is 2^-17 - 24 trees in bfloat16 204.7 us; cut instead 2^-16 and 203.8, and 0.35 % of the outputs round to a neighbour
+// of what the exact ones round to, not 0.19 %; one plane's 2^-8 would add as much error as rounding the result does); three for float32
 // are exact, as are the two or three planes of a float16 or float32 query.  Scores, statistics and sums are float32.
 //
 // What bounds it (8 key heads; calls one after the other): four sequences of 60 to 131 thousand keys of 128 in 8 bits, one token each, 169 us = 5.3 TB/s: the
@@ -122,8 +123,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r.u;
 }
 
-// eight floats as NP bf16 planes: all but the last cut, the last rounded
-template <int NP> __device__ __forceinline__ void split_planes(const float (&x)[8], Frag (&f)[NP]) {
+// eight floats as NP bf16 planes, the last rounded, the others cut or (NEAR) rounded too: the rest is half as large then, but a number next to the end
+// of the range would become infinite
+template <bool NEAR, int NP> __device__ __forceinline__ void split_planes(const float (&x)[8], Frag (&f)[NP]) {
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = x[j];
@@ -135,9 +137,9 @@ template <int NP> __device__ __forceinline__ void split_planes(const float (&x)[
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f[p].u[j] = __builtin_amdgcn_perm(__float_as_uint(y[2 * j + 1]), __float_as_uint(y[2 * j]), 0x07060302u);
-                y[2 * j] -= __uint_as_float(__float_as_uint(y[2 * j]) & 0xffff0000u);
-                y[2 * j + 1] -= __uint_as_float(__float_as_uint(y[2 * j + 1]) & 0xffff0000u);
+                f[p].u[j] = NEAR ? pack_bf16(y[2 * j], y[2 * j + 1]) : __builtin_amdgcn_perm(__float_as_uint(y[2 * j + 1]), __float_as_uint(y[2 * j]), 0x07060302u);
+                y[2 * j] -= __uint_as_float(NEAR ? f[p].u[j] << 16 : __float_as_uint(y[2 * j]) & 0xffff0000u);
+                y[2 * j + 1] -= __uint_as_float((NEAR ? f[p].u[j] : __float_as_uint(y[2 * j + 1])) & 0xffff0000u);
             }
         }
     }
@@ -394,10 +396,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                     for (int j = 0; j < 8; ++j) x[j] *= csign;
                     if constexpr (QLOW) {
                         Frag f[QP];
-                        split_planes<QP>(x, f);
+                        split_planes<false>(x, f);
                         q[rt][st][0] = f[0];
                         if (wave == 0) qlow[(rt * ST + st) * 64 + lane] = *reinterpret_cast<const kv_u32x4 *>(f[1].u);
-                    } else split_planes<QP>(x, q[rt][st]);
+                    } else split_planes<false>(x, q[rt][st]);
                 }
             }
         }
@@ -528,7 +530,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void tree_attention_kern
                 if (there != ~0u) kv.drop_values(there, g);
                 Frag pf[RT][PP];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) split_planes<PP>(p[rt], pf[rt]);
+                for (int rt = 0; rt < RT; ++rt) split_planes<PP == 2>(p[rt], pf[rt]);          // (three are exact either way)
 #pragma unroll
                 for (int w = 0; w < NB / TW; ++w) {
                     Frag vf[TW];

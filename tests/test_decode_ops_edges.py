@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from pero_ocr_amd import _native, decode_ops as ops
-from test_decode_ops import REPO, _check, _fake_pages, _gen, _problem
+from test_decode_ops import REPO, TYPES, _check, _fake_pages, _gen, _problem
 
 
 @pytest.mark.gpu
@@ -445,3 +445,34 @@ def test_gpu_attention_many_rows_all_types(dim, cache, kind):
     _check(few, kind, [t[:40] for t in got])
     for a, b in zip(got, ops.tree_attention(**dict(p, max_queries=0), want_lse=True)):
         assert torch.allclose(a.float(), b.float(), rtol=2 ** -7, atol=2 ** -7)          # the same sums in another order
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_gpu_probabilities_keep_seventeen_bits(kind):
+    """The weight of one key against values that take it away again.  Three keys with scores c < 0, 0, 0 and values 1, -x1, -x2, where x1 + x2 is e^c as
+    two bfloat16 numbers: out (2 + e^c) = e^c (1 + d) - x1 - x2, small enough for its own rounding not to hide d.  The kernel's e^c is
+    off by 4 u (1 + |c|) and as two planes by 2^-17; sums, divisions and the remaining roundings by a few u: |d| <= 2^-17 + 16 u (1 + |c|), and half a
+    step of the output's type on top."""
+    dim, tokens = 32, 400
+    dt = TYPES[kind]
+    c = (-torch.rand(tokens, device="cuda", generator=_gen(131)) * 4 - 2.0 ** -6).bfloat16()
+    want = torch.exp(c.double())
+    x1 = want.bfloat16()
+    x2 = (want - x1.double()).bfloat16()
+    pages = ops.kv_pages(tokens, 1, 16, dim, dtype="bf16")
+    pages.k[:, 0, 0, 0] = 1
+    for at, x in ((0, torch.ones_like(x1)), (1, -x1), (2, -x2)):
+        pages.v[:, 0, at] = x[:, None]
+    q = torch.zeros(tokens, 1, dim, device="cuda", dtype=dt)
+    q[:, 0, 0] = c.to(dt)
+    c = q[:, 0, 0].double()                                             # (float16 holds these eight bits too, or what it holds is the score)
+    want = torch.exp(c)
+    out = ops.tree_attention(q, pages, torch.arange(tokens, dtype=torch.int32, device="cuda")[:, None], torch.full((tokens,), 3, dtype=torch.int32, device="cuda"),
+                             torch.arange(tokens + 1, dtype=torch.int32, device="cuda"), scale=1.0, max_queries=1)
+    assert (out == out[:, :, :1]).all()
+    exact = (want - x1.double() - x2.double()) / (2 + want)
+    off = (out[:, 0, 0].double() - exact).abs()
+    allowed = want / (2 + want) * (2.0 ** -17 + 16 * 2.0 ** -24 * (1 + c.abs()))
+    half = torch.finfo(dt).eps / 2 * (exact.abs() + allowed) + (2.0 ** -25 if kind == "fp16" else 0)          # (float16 has fixed steps of 2^-24 below 2^-14)
+    assert (off <= allowed + half).all(), (off / (allowed + half)).max()
