@@ -25,7 +25,7 @@
 // probabilities) and conversions, which every wave repeats for its 32 rows, the rest waits for the address unit; one tree of 132 rows over 4129 keys of
 // 128 in 8 bits 18.3 us (5 or 6 blocks a wave, one on its way at a time) and 512 single tokens over 40 to 272 keys of 64, fp32, 25 us (2 to 9 blocks
 // a wave), where the start and the end of a workgroup (4 us) weigh most.  A chain takes all blocks of its sequence for every row tile and masks what lies
-// behind the tile's own tokens: 2048 new tokens, nothing before them, 32 heads over 8 of 128, 138 us for 57 us of products, of which the mask leaves half.
+// behind the tile's own tokens: 2048 new tokens, nothing before them, 32 heads over 8 of 128, 141 us for 57 us of products, of which the mask leaves half.
 //
 // A NaN or infinity in V spreads in a matrix product to the masked rows, whose probability is 0; testing every element for it costs more than the
 // transposition, so the loop does not.  Finite values near the end of the range may pass it in a sum of up to 2^8 times each, where the
